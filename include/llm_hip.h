@@ -40,7 +40,9 @@
 extern "C" {
 #endif
 
-#define LLH_ABI_VERSION 6  /* 6: head_dim-256 kernels, llh_metrics.d256_decode_calls / generic_decode_calls,
+#define LLH_ABI_VERSION 7  /* 7: query / key norms with rotation, attention weights, selection, compaction
+                              (new entry points only);
+                              6: head_dim-256 kernels, llh_metrics.d256_decode_calls / generic_decode_calls,
                               gate fields, LLH_KV_F16;
                               5: per-stream device error words, llh_layer_cache_create_from_rows;
                               4: int8 and fp8 pools store their scales as (K, V) pairs */
@@ -390,6 +392,141 @@ int llh_debug_decode_fp8(llh_ctx *ctx, const uint8_t *d_codes, float *d_out, int
  * reference rule on every f32 bit pattern but NaNs and stores how many codes differ
  * (a test hook, no reference counterpart; synchronous, allocates 8 bytes). */
 int llh_debug_fp8_encode_check(llh_ctx *ctx, uint64_t *h_mismatches);
+
+/* ------------------------------------------------------------------ */
+/* before the cache: norms and rotation of queries and keys            */
+/* ------------------------------------------------------------------ */
+
+/* How the rotated elements pair up: element i with i + rotary_dim / 2, or 2i with 2i + 1. */
+typedef enum llh_rope_pairs { LLH_ROPE_HALVES = 0, LLH_ROPE_ADJACENT = 1 } llh_rope_pairs;
+
+/* The rows of num_tokens new tokens and what turns them into queries and cached keys -- the
+ * steps the reference's callers take between the projections and attention (q/k RMSNorm, then
+ * RoPE, crates/llm-backend/src/core/qwen/ops/attention_full.rs:197-309):
+ *   y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset)      per head, over head_dim
+ *   (y_i, y_j) -> (y_i cos a - y_j sin a, y_j cos a + y_i sin a)  a = position * inv_freq[pair]
+ * over the pairs of the first rotary_dim elements.  All of it in f32, one rounding at the end;
+ * the angle's product and its reduction to one turn are in f64, so far positions lose nothing.
+ * Positions are given apart from cache slots: after an eviction they differ. */
+typedef struct llh_qk_rope_desc {
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;         /* at most 512 */
+  int32_t rotary_dim;       /* even, 0 (no rotation) .. head_dim */
+  int32_t pairs;            /* llh_rope_pairs */
+  float eps;
+  float weight_offset;      /* 0, or 1 for norms that multiply by 1 + weight */
+  int64_t q_stride;         /* elements from token to token (>= heads * head_dim): rows may lie side */
+  int64_t k_stride;         /* by side in a fused projection's output */
+  int64_t v_stride;
+  const void *d_q;          /* bf16, each token's [num_q_heads][head_dim] */
+  const void *d_k;          /* bf16, each token's [num_kv_heads][head_dim] */
+  const void *d_v;          /* the same; read by llh_qk_norm_rope_append only */
+  const void *d_q_weight;   /* bf16 [head_dim], or NULL: no norm (rotation alone) */
+  const void *d_k_weight;
+  const float *d_inv_freq;  /* [rotary_dim / 2] radians per position; unused when rotary_dim = 0 */
+  const int32_t *d_positions; /* [num_tokens]; unused when rotary_dim = 0 */
+} llh_qk_rope_desc;
+
+/* d_q_out [num_tokens][num_q_heads][head_dim], d_k_out [num_tokens][num_kv_heads][head_dim] bf16.
+ * d_q_out may be d_q, and d_k_out d_k, where those rows are contiguous (stride = heads *
+ * head_dim); no other overlap. */
+int llh_qk_norm_rope(llh_ctx *ctx, const llh_qk_rope_desc *desc, void *d_q_out, void *d_k_out, void *stream);
+/* The same, with the keys and the values written to the cache: the pool's bytes are those of
+ * llh_qk_norm_rope followed by llh_kv_append(d_slots, keys, values) (so a key is rounded to bf16
+ * before a quantised or fp16 pool's own rounding, and errors are flagged as there; slots of one
+ * call are distinct).  bf16 and fp16 pools take one launch; the others keep the rows in the
+ * stream's workspace between two.  num_kv_heads and head_dim must be the pool's. */
+int llh_qk_norm_rope_append(llh_ctx *ctx, llh_kv_pool *pool, const llh_qk_rope_desc *desc, const int64_t *d_slots,
+                            void *d_q_out, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* attention that says where its weight went, and eviction by it       */
+/* ------------------------------------------------------------------ */
+
+/* One decode step that also accumulates the softmax weight each cached token received:
+ *   weights_out[b][kvh][p] = decay * weights_in[b][kvh][p]
+ *                            + sum over the kv head's query heads of weight p    for p < len_b
+ * (tokens outside the window receive 0; entries from len_b on are left as they were).
+ * d_weights_in, d_weights_out: f32 [num_seqs][kv_heads][weights_stride], weights_stride >=
+ * max_seq_len.  d_weights_in = NULL stands for zeros; it may be d_weights_out, no other overlap.
+ * decay must be finite.  The output is llh_paged_decode's within the rounding of the weights;
+ * every pool format, head_dim <= 512.  A key in a block outside the pool is masked (and flagged),
+ * a query that is left with no key gives a zero row and adds nothing, and a non-finite score
+ * is flagged.  A sequence that is flagged for its length gets neither output nor weights.
+ * The scores pass through the stream's workspace: llh_weights_workspace_bytes. */
+int llh_paged_decode_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_decode_desc *desc, const void *d_q,
+                             void *d_out, float score_scale, const float *d_weights_in, float *d_weights_out,
+                             int64_t weights_stride, float decay, void *stream);
+/* The same for the last rows of each sequence (a short prefill chunk, or the last rows of a
+ * prompt as observers of all of it): attention of llh_paged_prefill, the weights summed over the
+ * sequence's query rows too (a sequence without rows adds nothing: weights_out = decay *
+ * weights_in).  max_chunk_len is at most LLH_WEIGHTS_MAX_CHUNK (else LLH_ERR_UNSUPPORTED);
+ * max_context_len bounds d_context_lens. */
+#define LLH_WEIGHTS_MAX_CHUNK 64
+int llh_paged_prefill_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_prefill_desc *desc,
+                              int32_t max_context_len, const void *d_q, void *d_out, float score_scale,
+                              const float *d_weights_in, float *d_weights_out, int64_t weights_stride, float decay,
+                              void *stream);
+/* Workspace bytes of either call (max_chunk_len = 1: a decode step), for any split. */
+size_t llh_weights_workspace_bytes(int32_t num_seqs, int32_t max_chunk_len, int32_t num_q_heads, int32_t head_dim,
+                                   int32_t max_context_len);
+
+/* Which tokens to keep.  For each (sequence, kv head), of len_b tokens: all of them when
+ * len_b <= budget, else the first `sinks`, the last `recent`, and of the others those of the
+ * largest weights, budget in all; equal weights (0 and -0 are equal) go to the lowest position,
+ * a NaN counts below every number.
+ *   d_weights f32 [num_seqs][kv_heads][weights_stride]
+ *   d_keep    int32 [num_seqs][kv_heads][keep_stride]: the kept positions, ascending; entries
+ *             from min(len_b, budget) on are left as they were
+ *   d_kept_lens int32 [num_seqs]: min(len_b, budget) -- the sequence's length after llh_kv_compact;
+ *             not d_seq_lens itself
+ * A length above max_seq_len is flagged (2), keeps nothing and reports 0.  Rows of more than 32768
+ * positions keep counts in the stream's workspace. */
+typedef struct llh_kv_select_desc {
+  int32_t num_seqs;
+  int32_t kv_heads;
+  int32_t max_seq_len;     /* host-known bound on d_seq_lens, <= weights_stride */
+  int32_t budget;          /* >= 1 */
+  int32_t sinks;           /* >= 0 */
+  int32_t recent;          /* >= 0; sinks + recent <= budget */
+  int64_t weights_stride;
+  int64_t keep_stride;     /* >= min(budget, max_seq_len) */
+  const int32_t *d_seq_lens;
+} llh_kv_select_desc;
+int llh_kv_select(llh_ctx *ctx, const llh_kv_select_desc *desc, const float *d_weights, int32_t *d_keep,
+                  int32_t *d_kept_lens, void *stream);
+
+/* Moves the kept tokens to the front of other blocks: token i of kv head h of sequence b becomes
+ * the one at position d_keep[b][h][i] (each head keeps its own), for i < d_kept_lens[b], and with
+ * it its accumulated weight.  Slots of the last destination block past the kept tokens are zeroed.
+ * Codes and scales of int8 pools are moved; fp8 blocks, whose scale spans the block, are encoded
+ * anew from the dequantised rows by the rule of llh_kv_write_blocks (a token whose block's scale
+ * stays keeps its codes); LLH_KV_INT8_ROW pools are LLH_ERR_UNSUPPORTED (one scale per token spans
+ * all heads, which keep different tokens).
+ * Destination blocks must not be among the call's source blocks, nor named twice.  A position
+ * that is negative, at or past the sequence's length, its table row or weights_in_stride, and a
+ * source block outside the pool, are flagged (1) and leave a zero token; a destination block
+ * outside the pool is flagged (1) and skipped; a kept length above max_kept is flagged (2)
+ * and its sequence is left alone. */
+typedef struct llh_kv_compact_desc {
+  int32_t num_seqs;
+  int32_t max_kept;        /* host-known bound on d_kept_lens, <= keep_stride, dst_max_blocks * block_tokens */
+  int32_t src_max_blocks;  /* row stride of d_src_tables */
+  int32_t dst_max_blocks;  /* row stride of d_dst_tables */
+  int64_t keep_stride;
+  int64_t weights_in_stride;
+  int64_t weights_out_stride;   /* >= max_kept */
+  const int32_t *d_seq_lens;    /* [num_seqs] lengths before */
+  const int32_t *d_kept_lens;   /* [num_seqs] lengths after */
+  const int32_t *d_keep;        /* [num_seqs][kv_heads][keep_stride] */
+  const int32_t *d_src_tables;  /* [num_seqs][src_max_blocks] */
+  const int32_t *d_dst_tables;  /* [num_seqs][dst_max_blocks] */
+  const float *d_weights_in;    /* [num_seqs][kv_heads][weights_in_stride], or NULL (both) */
+  float *d_weights_out;         /* [num_seqs][kv_heads][weights_out_stride]; no overlap with the input */
+} llh_kv_compact_desc;
+int llh_kv_compact(llh_ctx *ctx, llh_kv_pool *pool, const llh_kv_compact_desc *desc, void *stream);
 
 /* ------------------------------------------------------------------ */
 /* trait mirror: LayerKvCache + NativeMatvecBackend attention hooks    */

@@ -1331,6 +1331,160 @@ int llh_paged_prefill(llh_ctx *ctx, const llh_kv_pool *pool, const llh_prefill_d
   return LLH_OK;
 }
 
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// attention with accumulated weights
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// One call of either kind: a decode step (chunk_starts null, one row per sequence) or the last
+// rows of each sequence.  max_ctx bounds the context lengths, total_hint the attended tokens.
+struct WeightsCall {
+  int32_t num_seqs, max_rows, q_heads, max_blocks, window, max_ctx, total_hint;
+  const int32_t *chunk_starts, *lens, *tables;
+  const void *gate;
+};
+
+// Positions a score row may hold: the span, behind the multiple of 64 it starts from, in whole
+// units of 64 keys.
+int64_t score_stride(int64_t span) { return (span + 63) / 64 * 64 + 64; }
+
+int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, const void *d_q, void *d_out,
+                 float score_scale, const float *d_in, float *d_w, int64_t stride, float decay, void *stream) {
+  if (!d_q || !d_out || !d_w || !c.lens || !c.tables)
+    return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
+  if (c.num_seqs > 65535) return ctx->fail(LLH_ERR_INVALID_SHAPE, "num_seqs must be <= 65535");
+  if (stride < std::max(1, c.max_ctx))
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "weights_stride must hold the longest context");
+  if ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 1)
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "q and output must be bf16-aligned (2 bytes)");
+  if ((reinterpret_cast<uintptr_t>(d_in) | reinterpret_cast<uintptr_t>(d_w)) & 3)
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "weights must be f32-aligned (4 bytes)");
+  if (!std::isfinite(score_scale) || !std::isfinite(decay))
+    return ctx->fail(LLH_ERR_NON_FINITE, "score scale and decay must be finite");
+  const PoolView &pv = pool->view;
+  if (pv.head_dim > kWeightsMaxDim) {
+    ctx->not_handled++;
+    return ctx->fail(LLH_ERR_UNSUPPORTED, "attention weights take head_dim <= " + std::to_string(kWeightsMaxDim));
+  }
+  const bool tuned = pv.format != LLH_KV_INT8_ROW && (pv.head_dim == kFastHeadDim || pv.head_dim == kD256HeadDim) &&
+                     pv.block_tokens == kFastBlockTokens && aligned16(d_q) && aligned16(d_out) &&
+                     !ctx->opt(LLH_OPT_FORCE_GENERIC);
+  const int64_t span = std::max<int64_t>(
+      1, c.window > 0 ? std::min<int64_t>((int64_t)c.window + c.max_rows - 1, c.max_ctx) : c.max_ctx);
+  const size_t rows = (size_t)c.num_seqs * c.max_rows * c.q_heads;
+  SplitRows sr{};
+  if (tuned) {
+    const int group = c.q_heads / pv.kv_heads;
+    const int uk = rows_unit_keys(pv.head_dim);
+    const int units = (int)((span + uk - 1) / uk) + (c.window > 0 ? 1 : 0);
+    const long long tiles = ((long long)c.max_rows * group + 15) / 16 * pv.kv_heads;
+    const long long total =
+        c.total_hint > 0 ? tiles * ((long long)c.total_hint / uk + c.num_seqs) : tiles * units * c.num_seqs;
+    sr = split_rows(ctx, pv, tiles * c.num_seqs, units, total, rows, SIZE_MAX);
+  }
+  const size_t ml_off = sr.bytes;
+  const size_t sc_off = ml_off + align_up(rows * sizeof(float2));
+  const int64_t sc_stride = score_stride(span);
+  if (sc_stride > INT32_MAX) return ctx->fail(LLH_ERR_INVALID_SHAPE, "context too long for one call");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  WsLease lease;
+  const int st = lease.acquire(ctx, s, sc_off + rows * sc_stride * sizeof(float));
+  if (st != LLH_OK) return st;
+  WeightsArgs w{};
+  RowsArgs &r = w.rows;
+  r.pool = pv;
+  r.q = static_cast<const uint16_t *>(d_q);
+  r.out = static_cast<uint16_t *>(d_out);
+  r.chunk_starts = c.chunk_starts;
+  r.context_lens = c.lens;
+  r.tables = c.tables;
+  r.ws_ml = reinterpret_cast<float2 *>(lease.base());
+  r.ws_o = reinterpret_cast<float *>(lease.base() + sr.o_off);
+  r.err = lease.err();
+  r.num_seqs = c.num_seqs;
+  r.max_rows = c.max_rows;
+  r.q_heads = c.q_heads;
+  r.max_blocks = c.max_blocks;
+  r.window = c.window;
+  r.split_units = std::max(1, sr.split_units);
+  r.max_splits = std::max(1, sr.max_splits);
+  r.single_units = sr.single_units;
+  r.max_span = (int32_t)span;
+  r.max_len = std::max(1, c.max_ctx);
+  r.flag_nonfinite = 1;
+  r.scale = score_scale;
+  r.scale_log2e = score_scale * 1.4426950408889634f;
+  r.gate = static_cast<const uint16_t *>(c.gate);
+  r.row_ml = reinterpret_cast<float2 *>(lease.base() + ml_off);
+  r.scores = reinterpret_cast<float *>(lease.base() + sc_off);
+  r.score_stride = (int32_t)sc_stride;
+  w.w_in = d_in;
+  w.w_out = d_w;
+  w.stride = stride;
+  w.decay = decay;
+  (c.chunk_starts ? ctx->prefill_calls : ctx->decode_calls)++;
+  if (tuned) ctx->routes[c.chunk_starts ? LLH_ROUTE_ROWS_PREFILL : LLH_ROUTE_ROWS_DECODE]++;
+  else (c.chunk_starts ? ctx->generic_prefill_calls : ctx->generic_decode_calls)++;
+  hipError_t e = tuned ? launch_rows(r, false, s) : launch_weights_generic(r, s);
+  if (e == hipSuccess) e = launch_weights_accumulate(w, c.max_ctx, s);
+  if (e != hipSuccess) return ctx->hip_fail(e, "attention weights launch");
+  return LLH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t llh_weights_workspace_bytes(int32_t num_seqs, int32_t max_chunk_len, int32_t num_q_heads, int32_t head_dim,
+                                   int32_t max_context_len) {
+  if (num_seqs <= 0 || max_chunk_len <= 0 || num_q_heads <= 0 || head_dim <= 0 || max_context_len < 0) return 0;
+  const size_t rows = (size_t)num_seqs * max_chunk_len * num_q_heads;
+  // split_rows: at most four splits a workgroup slot, 16 rows each
+  const size_t partial = std::min<size_t>(rows * kRowsMaxSplits, (size_t)64 * 1024);
+  return align_up(partial * sizeof(float2)) + align_up(partial * head_dim * sizeof(float)) + kAlign +
+         align_up(rows * sizeof(float2)) + rows * score_stride(std::max(1, max_context_len)) * sizeof(float);
+}
+
+int llh_paged_decode_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_decode_desc *desc, const void *d_q,
+                             void *d_out, float score_scale, const float *d_weights_in, float *d_weights_out,
+                             int64_t weights_stride, float decay, void *stream) {
+  if (!ctx || !pool || !desc) return LLH_ERR_NULL;
+  int st = check_desc_common(ctx, pool, desc->num_seqs, desc->num_q_heads, desc->max_blocks_per_seq, desc->window);
+  if (st != LLH_OK || desc->num_seqs == 0) return st;
+  if (desc->max_seq_len < 0) return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_seq_len must be >= 0");
+  st = check_span(ctx, pool, desc->max_seq_len, desc->window, desc->max_blocks_per_seq);
+  if (st != LLH_OK) return st;
+  const WeightsCall c{desc->num_seqs, 1, desc->num_q_heads, desc->max_blocks_per_seq, desc->window, desc->max_seq_len,
+                      desc->total_tokens_hint, nullptr, desc->d_seq_lens, desc->d_block_tables, desc->d_gate};
+  return weights_impl(ctx, pool, c, d_q, d_out, score_scale, d_weights_in, d_weights_out, weights_stride, decay,
+                      stream);
+}
+
+int llh_paged_prefill_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_prefill_desc *desc,
+                              int32_t max_context_len, const void *d_q, void *d_out, float score_scale,
+                              const float *d_weights_in, float *d_weights_out, int64_t weights_stride, float decay,
+                              void *stream) {
+  if (!ctx || !pool || !desc) return LLH_ERR_NULL;
+  int st = check_desc_common(ctx, pool, desc->num_seqs, desc->num_q_heads, desc->max_blocks_per_seq, desc->window);
+  if (st != LLH_OK || desc->num_seqs == 0) return st;
+  if (desc->total_q_rows < 0 || desc->max_chunk_len <= 0 || max_context_len < 0)
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "row counts must be >= 0 and chunks at least one row");
+  if (desc->max_chunk_len > LLH_WEIGHTS_MAX_CHUNK) {
+    ctx->not_handled++;
+    return ctx->fail(LLH_ERR_UNSUPPORTED,
+                     "attention weights take at most " + std::to_string(LLH_WEIGHTS_MAX_CHUNK) + " rows a sequence");
+  }
+  if (!desc->d_chunk_starts) return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
+  const WeightsCall c{desc->num_seqs, desc->max_chunk_len, desc->num_q_heads, desc->max_blocks_per_seq, desc->window,
+                      max_context_len, 0, desc->d_chunk_starts, desc->d_context_lens, desc->d_block_tables,
+                      desc->d_gate};
+  return weights_impl(ctx, pool, c, d_q, d_out, score_scale, d_weights_in, d_weights_out, weights_stride, decay,
+                      stream);
+}
+
 int llh_debug_gather(llh_ctx *ctx, const llh_kv_pool *pool, const llh_decode_desc *desc, int32_t seq, int32_t lo,
                      int32_t hi, int32_t tensor, void *d_out, void *stream) {
   if (!ctx || !pool || !desc) return LLH_ERR_NULL;

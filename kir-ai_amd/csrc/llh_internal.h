@@ -177,8 +177,62 @@ struct RowsArgs {
   float scale;
   float scale_log2e;
   const uint16_t *gate;
+  // attention weights (weights.hip): null, or [num_seqs][max_rows][Hq][score_stride] scores in
+  // log2 units, position p at p - weights_base(first attended position), and the (max, sum) of each row
+  float *scores;
+  float2 *row_ml;           // [num_seqs][max_rows][Hq]
+  int32_t score_stride;     // a multiple of 64
 };
 int rows_unit_keys(int head_dim);
+// Scores are stored from a multiple of 64 positions on, so that units and vectors of keys are whole.
+__host__ __device__ constexpr int weights_base(int lo) { return lo & ~63; }
+
+// Accumulation of the softmax weights over the rows of `rows` (its scores and row_ml).
+struct WeightsArgs {
+  RowsArgs rows;
+  const float *w_in;        // [num_seqs][Hkv][stride], or null (zeros)
+  float *w_out;
+  int64_t stride;
+  float decay;
+};
+
+// Norms and rotation of queries and keys (qkrope.hip).
+struct QkRopeArgs {
+  const uint16_t *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  const uint16_t *q_weight, *k_weight;  // null: no norm
+  const float *inv_freq;
+  const int32_t *positions;
+  uint16_t *q_out;          // [n][Hq][D]
+  uint16_t *k_out, *v_out;  // [n][Hkv][D], or null: into the pool (bf16, fp16) at slots; v_out null beside k_out: no values
+  const int64_t *slots;
+  PoolView pool;
+  void *k_dst, *v_dst;
+  int32_t *err;
+  int32_t n, q_heads, kv_heads, head_dim, rotary_dim, adjacent;
+  float eps, offset;
+};
+constexpr int kRopeMaxDim = 512;
+
+struct SelectArgs {
+  const float *weights;
+  const int32_t *seq_lens;
+  int32_t *keep, *kept_lens;
+  int64_t weights_stride, keep_stride;
+  int32_t *err;
+  int32_t num_seqs, kv_heads, max_seq_len, budget, sinks, recent;
+};
+
+struct CompactArgs {
+  PoolView pool;
+  void *k_dst, *v_dst, *ks_dst, *vs_dst;
+  const int32_t *seq_lens, *kept_lens, *keep, *src_tables, *dst_tables;
+  const float *w_in;
+  float *w_out;
+  int64_t keep_stride, w_in_stride, w_out_stride;
+  int32_t *err;
+  int32_t num_seqs, max_kept, src_max_blocks, dst_max_blocks;
+};
 
 struct WriteBlocksArgs {
   PoolView pool;
@@ -285,5 +339,12 @@ hipError_t launch_decode_fp8(const uint8_t *codes, float *out, int32_t n, hipStr
 // encoder differs from the integer reference rule
 hipError_t launch_fp8_encode_check(unsigned long long *mismatches, hipStream_t s);
 hipError_t launch_matvec_bf16(const MatvecArgs &a, hipStream_t s);
+// scores, row_ml and output of every shape the packed-row kernel does not take (head_dim <= 512)
+constexpr int kWeightsMaxDim = 512;
+hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s);
+hipError_t launch_weights_accumulate(const WeightsArgs &a, int max_len, hipStream_t s);
+hipError_t launch_qk_rope(const QkRopeArgs &a, hipStream_t s);
+hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s);
+hipError_t launch_kv_compact(const CompactArgs &a, hipStream_t s);
 
 }  // namespace llh

@@ -47,6 +47,7 @@
 // Hq16 / Hkv2, head_dim 256, int8: 10.6 ms element-wise, 48 us here (197 TFLOP/s: the code
 // conversions, repeated by every 16-row tile, bound it).
 #include "arrival.h"
+#include "rows_split.h"
 
 namespace llh {
 
@@ -110,42 +111,11 @@ __device__ __forceinline__ void f16x8_to_bf16(const u32x4_t &w, u32x4_t &hi, u32
   }
 }
 
-// The keys of a sequence and their split, the same in every kernel of a call.
-struct SeqSplit {
-  int c0, chunk, ctx;  // first query row, query rows, context length
-  int lo;              // first position any row attends
-  int unit0, units;    // units of UK keys
-  int per_split, n_splits;
-  bool skip;           // nothing to compute (flags: why)
-  int flags;
-};
-
-template <int UK>
-__device__ __forceinline__ SeqSplit seq_split(const RowsArgs &a, int b) {
-  SeqSplit s;
-  s.flags = 0;
-  s.c0 = a.chunk_starts ? a.chunk_starts[b] : b;
-  s.chunk = a.chunk_starts ? a.chunk_starts[b + 1] - s.c0 : 1;
-  s.ctx = a.context_lens[b];
-  const int first = s.ctx - s.chunk;  // position of the first row
-  s.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  const int span = max(0, s.ctx - s.lo);
-  if ((a.max_span > 0 && span > a.max_span) || (a.max_len > 0 && s.ctx > a.max_len)) s.flags = kErrTooManySplits;
-  else if ((int64_t)span > (int64_t)a.max_blocks * BT) s.flags = kErrSpan;
-  s.skip = s.flags != 0 || s.chunk <= 0 || (a.chunk_starts && s.ctx < s.chunk);
-  s.unit0 = s.lo / UK;
-  s.units = span > 0 ? (s.ctx - 1) / UK - s.unit0 + 1 : 0;
-  s.per_split = s.units <= a.single_units ? a.single_units
-                                          : max(a.split_units, (s.units + a.max_splits - 1) / a.max_splits);
-  s.n_splits = (s.units + s.per_split - 1) / s.per_split;
-  return s;
-}
-
 // 1 / (weight sum).  No weight at all (every key masked, or every score -inf) gives the zero
 // row of the tile prefill and the reference-order decode, and the NaN (0 / 0) of the vector
 // decode kernels in the calls that are theirs too.
 __device__ __forceinline__ float row_inv(const RowsArgs &a, float ll) {
-  return ll == 0.0f && (a.chunk_starts || a.zero_bad) ? 0.0f : 1.0f / ll;
+  return ll == 0.0f && (a.chunk_starts || a.zero_bad || a.scores) ? 0.0f : 1.0f / ll;
 }
 
 // keys per unit: K and V of a unit take 64 operand registers each in 16-bit formats (32 in
@@ -196,8 +166,10 @@ __device__ __forceinline__ void merge_splits(const RowsArgs &a, const SeqSplit &
   }
 }
 
-template <int D, int FMT, int PARTS>
+// SCORES: every score and each row's (max, sum) are stored for weights.hip.
+template <int D, int FMT, int PARTS, bool SCORES = false>
 __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void paged_rows_kernel(const RowsArgs a) {
+  static_assert(!SCORES || PARTS > 1 || !is16(FMT), "the sum is that of the weights before any rounding");
   constexpr bool Q8 = !is16(FMT);
   constexpr bool WIDE16 = FMT == kF16 && PARTS == 3;  // fp16 elements as two bf16 terms
   constexpr int OP = FMT == kF16 && !WIDE16 ? kF16 : kBf16;
@@ -426,6 +398,15 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
       sc[x] = on ? s * c : -INFINITY;
       tmax = fmaxf(tmax, sc[x]);
     }
+    if constexpr (SCORES) {
+      if (row0 + col < rows) {
+        float *to = a.scores + (((size_t)b * a.max_rows + my_tok) * a.q_heads + kvh * G + my_row % G) * a.score_stride +
+                    (base - weights_base(sq.lo));
+#pragma unroll
+        for (int x = 0; x < 4 * NT; x += 4)
+          *reinterpret_cast<f32x4_t *>(to + key_of(x)) = f32x4_t{sc[x], sc[x + 1], sc[x + 2], sc[x + 3]};
+      }
+    }
     tmax = fmaxf(tmax, xor16_other(tmax, lane));
     tmax = fmaxf(tmax, xor32_other(tmax, lane));
     // lazy rescale: the reference max moves only when a row's max grows by more than 8
@@ -593,6 +574,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
     const int head = kvh * G + (row0 + r) % G;
     if (sq.n_splits == 1) {
       const float inv = row_inv(a, ll);
+      if constexpr (SCORES) {
+        if (d == 0) a.row_ml[((size_t)b * a.max_rows + tok) * a.q_heads + head] = make_float2(mm, ll);
+      }
       const size_t o = ((size_t)(sq.c0 + tok) * a.q_heads + head) * D + d;
 #pragma unroll
       for (int x = 0; x < 4; x++) a.out[o + x] = f32_to_bf16_rne(gated(oo[x] * inv, a.gate, o + x));
@@ -640,8 +624,9 @@ __device__ __forceinline__ void rows_merge(const RowsArgs &a, size_t prow, size_
   const int li = d & 63;
   const float2 ml = a.ws_ml[p0 + min(li, last)];
   const float mx[1] = {li <= last ? ml.x : -INFINITY}, ly[1] = {ml.y};
-  float f[1];
-  const float ll = merge_weights<1>(mx, ly, li, f);
+  float f[1], top;
+  const float ll = merge_weights<1>(mx, ly, li, f, &top);
+  if (a.row_ml && d == 0) a.row_ml[prow] = make_float2(top, ll);
   float oo = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; i++)  // nothing of the places past the last (0 x infinity is NaN)
@@ -666,11 +651,11 @@ __global__ __launch_bounds__(D) void paged_rows_merge_kernel(const RowsArgs a) {
   return rows_merge<D, kRowsMaxSplits>(a, prow, orow, last, d);
 }
 
-template <int D, int FMT, int PARTS>
+template <int D, int FMT, int PARTS, bool SCORES = false>
 hipError_t launch_rows_t(const RowsArgs &a, hipStream_t s, void *hu, LaunchHook hook) {
   const unsigned tiles = (unsigned)(((long long)a.max_rows * (a.q_heads / a.pool.kv_heads) + TILE - 1) / TILE);
   if (hook) hook(hu, 0, s);
-  hipLaunchKernelGGL((paged_rows_kernel<D, FMT, PARTS>), dim3(tiles * a.pool.kv_heads, a.num_seqs, a.max_splits),
+  hipLaunchKernelGGL((paged_rows_kernel<D, FMT, PARTS, SCORES>), dim3(tiles * a.pool.kv_heads, a.num_seqs, a.max_splits),
                      dim3(64 * WAVES), 0, s, a);
   hipError_t e = hipGetLastError();
   if (hook) hook(hu, 1, s);
@@ -694,6 +679,18 @@ hipError_t launch_rows_16(const RowsArgs &a, bool exact_weights, hipStream_t s, 
 
 template <int D>
 hipError_t launch_rows_d(const RowsArgs &a, bool exact_weights, hipStream_t s, void *hu, LaunchHook hook) {
+  if (a.scores) switch (a.pool.format) {
+    case kBf16:
+      return launch_rows_t<D, kBf16, 2, true>(a, s, hu, hook);
+    case kF16:
+      return launch_rows_t<D, kF16, 2, true>(a, s, hu, hook);
+    case kInt8:
+      return launch_rows_t<D, kInt8, 3, true>(a, s, hu, hook);
+    case kFp8:
+      return launch_rows_t<D, kFp8, 3, true>(a, s, hu, hook);
+    default:
+      return hipErrorInvalidValue;
+  }
   switch (a.pool.format) {
     case kBf16:
       return launch_rows_16<D, kBf16>(a, exact_weights, s, hu, hook);

@@ -108,6 +108,67 @@ class PrefillDesc(ctypes.Structure):
     ]
 
 
+ROPE_HALVES = 0    # element i turns with element i + rotary_dim / 2
+ROPE_ADJACENT = 1  # element 2i with 2i + 1
+WEIGHTS_MAX_CHUNK = 64
+
+
+class QkRopeDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_tokens", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("weight_offset", ctypes.c_float),
+        ("q_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64),
+        ("d_q", ctypes.c_void_p),
+        ("d_k", ctypes.c_void_p),
+        ("d_v", ctypes.c_void_p),
+        ("d_q_weight", ctypes.c_void_p),
+        ("d_k_weight", ctypes.c_void_p),
+        ("d_inv_freq", ctypes.c_void_p),
+        ("d_positions", ctypes.c_void_p),
+    ]
+
+
+class KvSelectDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_seqs", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("max_seq_len", ctypes.c_int32),
+        ("budget", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("weights_stride", ctypes.c_int64),
+        ("keep_stride", ctypes.c_int64),
+        ("d_seq_lens", ctypes.c_void_p),
+    ]
+
+
+class KvCompactDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_seqs", ctypes.c_int32),
+        ("max_kept", ctypes.c_int32),
+        ("src_max_blocks", ctypes.c_int32),
+        ("dst_max_blocks", ctypes.c_int32),
+        ("keep_stride", ctypes.c_int64),
+        ("weights_in_stride", ctypes.c_int64),
+        ("weights_out_stride", ctypes.c_int64),
+        ("d_seq_lens", ctypes.c_void_p),
+        ("d_kept_lens", ctypes.c_void_p),
+        ("d_keep", ctypes.c_void_p),
+        ("d_src_tables", ctypes.c_void_p),
+        ("d_dst_tables", ctypes.c_void_p),
+        ("d_weights_in", ctypes.c_void_p),
+        ("d_weights_out", ctypes.c_void_p),
+    ]
+
+
 class PoolInfo(ctypes.Structure):
     _fields_ = [
         ("format", ctypes.c_int32),
@@ -320,6 +381,15 @@ SIGNATURES = {
     "llh_paged_decode_append": (ctypes.c_int, [_P, _P, ctypes.POINTER(DecodeDesc), _P, _P, _P, _P, ctypes.c_float,
                                                _P]),
     "llh_paged_prefill": (ctypes.c_int, [_P, _P, ctypes.POINTER(PrefillDesc), _P, _P, ctypes.c_float, _P]),
+    "llh_qk_norm_rope": (ctypes.c_int, [_P, ctypes.POINTER(QkRopeDesc), _P, _P, _P]),
+    "llh_qk_norm_rope_append": (ctypes.c_int, [_P, _P, ctypes.POINTER(QkRopeDesc), _P, _P, _P]),
+    "llh_paged_decode_weights": (ctypes.c_int, [_P, _P, ctypes.POINTER(DecodeDesc), _P, _P, ctypes.c_float, _P, _P,
+                                                ctypes.c_int64, ctypes.c_float, _P]),
+    "llh_paged_prefill_weights": (ctypes.c_int, [_P, _P, ctypes.POINTER(PrefillDesc), _I32, _P, _P, ctypes.c_float, _P,
+                                                 _P, ctypes.c_int64, ctypes.c_float, _P]),
+    "llh_weights_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "llh_kv_select": (ctypes.c_int, [_P, ctypes.POINTER(KvSelectDesc), _P, _P, _P, _P]),
+    "llh_kv_compact": (ctypes.c_int, [_P, _P, ctypes.POINTER(KvCompactDesc), _P]),
     "llh_debug_gather": (ctypes.c_int, [_P, _P, ctypes.POINTER(DecodeDesc), _I32, _I32, _I32, _I32, _P, _P]),
     "llh_debug_decode_fp8": (ctypes.c_int, [_P, _P, _P, _I32, _P]),
     "llh_debug_fp8_encode_check": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_uint64)]),
@@ -587,13 +657,13 @@ class Context:
     def bind(self, name: str, *args):
         """A zero-argument call of the C entry point `name` with the context handle and the
         given arguments converted to ctypes values once (device tensors become their
-        pointers, DecodeDesc / PrefillDesc are passed by reference, streams by handle), for
+        pointers, descriptors are passed by reference, streams by handle), for
         loops that issue the same call many times: the per-call Python work is one C call and
         the status check.  The tensors and descriptors must outlive the returned call."""
         fn = getattr(self.lib, name)
         conv = [self.handle]
         for a in args:
-            if isinstance(a, (DecodeDesc, PrefillDesc)):
+            if isinstance(a, ctypes.Structure):
                 conv.append(ctypes.byref(a))
             elif isinstance(a, (KvPool, LayerKvCache)):
                 conv.append(a.handle)
@@ -648,6 +718,139 @@ class Context:
                 self.handle, pool.handle, ctypes.byref(desc), _ptr(q), _ptr(out), score_scale, _stream(stream)
             )
         )
+
+    # ---- before the cache, and eviction from it ----
+    @staticmethod
+    def qk_rope_desc(q, k, v, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6,
+                     weight_offset: float = 0.0, adjacent: bool = False) -> QkRopeDesc:
+        """Descriptor over bf16 [tokens][heads][head_dim] tensors, which may be views of a fused projection's
+        rows (any token stride, heads side by side); v: None, or the values that go to the cache.  positions:
+        int32 [tokens]; inv_freq: f32 [rotary_dim / 2], or None for no rotation (positions may then be None).
+        It keeps the tensors alive (it stores raw pointers)."""
+        import torch
+
+        for x in (q, k, v):
+            if x is None:
+                continue
+            if x.dim() != 3 or (x.shape[1] > 1 and x.stride(1) != x.shape[2]) or (x.shape[2] > 1 and x.stride(2) != 1):
+                raise LlhError(ERR_INVALID_SHAPE, "rows are [tokens][heads][head_dim] with a token's heads side by side")
+            if x.dtype not in (torch.bfloat16, torch.int16, torch.uint16):
+                raise LlhError(ERR_UNSUPPORTED, "rows are bf16")
+        if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or (v is not None and v.shape != k.shape):
+            raise LlhError(ERR_INVALID_SHAPE, "queries, keys and values of the same tokens and head_dim")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.numel() != q.shape[2] or not w.is_contiguous()):
+                raise LlhError(ERR_INVALID_SHAPE, "norm weights are [head_dim]")
+        if inv_freq is not None and inv_freq.dtype != torch.float32:
+            raise LlhError(ERR_UNSUPPORTED, "inv_freq is f32")
+        if positions is not None and (positions.dtype != torch.int32 or positions.numel() != q.shape[0]):
+            raise LlhError(ERR_INVALID_SHAPE, "positions are int32 [tokens]")
+        # a token's stride is read only from the second token on
+        stride = lambda x: max(x.stride(0), x.shape[1] * x.shape[2]) if x.shape[0] <= 1 else x.stride(0)
+        d = QkRopeDesc(
+            num_tokens=q.shape[0],
+            num_q_heads=q.shape[1],
+            num_kv_heads=k.shape[1],
+            head_dim=q.shape[2],
+            rotary_dim=0 if inv_freq is None else 2 * inv_freq.numel(),
+            pairs=ROPE_ADJACENT if adjacent else ROPE_HALVES,
+            eps=eps,
+            weight_offset=weight_offset,
+            q_stride=stride(q),
+            k_stride=stride(k),
+            v_stride=0 if v is None else stride(v),
+            d_q=_ptr(q),
+            d_k=_ptr(k),
+            d_v=_ptr(v),
+            d_q_weight=_ptr(q_weight),
+            d_k_weight=_ptr(k_weight),
+            d_inv_freq=_ptr(inv_freq),
+            d_positions=_ptr(positions),
+        )
+        d._keep = (q, k, v, positions, inv_freq, q_weight, k_weight)
+        return d
+
+    def qk_norm_rope(self, desc: QkRopeDesc, q_out, k_out, stream=None) -> None:
+        """llh_qk_norm_rope: per-head norms and rotation of queries and keys."""
+        self.check(self.lib.llh_qk_norm_rope(self.handle, ctypes.byref(desc), _ptr(q_out), _ptr(k_out),
+                                             _stream(stream)))
+
+    def qk_norm_rope_append(self, pool: "KvPool", desc: QkRopeDesc, slots, q_out, stream=None) -> None:
+        """llh_qk_norm_rope_append: the same, with keys and values written to the pool's slots (int64 [tokens])."""
+        self.check(self.lib.llh_qk_norm_rope_append(self.handle, pool.handle, ctypes.byref(desc), _ptr(slots),
+                                                    _ptr(q_out), _stream(stream)))
+
+    def paged_decode_weights(self, pool: "KvPool", desc: DecodeDesc, q, out, score_scale: float, weights_in,
+                             weights_out, decay: float = 1.0, stream=None) -> None:
+        """llh_paged_decode_weights: a decode step that adds each token's softmax weight to the accumulator,
+        f32 [num_seqs][kv_heads][stride]; weights_in: None (zeros), another tensor or weights_out itself."""
+        self._check_weights(weights_in, weights_out)
+        self.check(self.lib.llh_paged_decode_weights(
+            self.handle, pool.handle, ctypes.byref(desc), _ptr(q), _ptr(out), score_scale, _ptr(weights_in),
+            _ptr(weights_out), weights_out.shape[-1], decay, _stream(stream)))
+
+    def paged_prefill_weights(self, pool: "KvPool", desc: PrefillDesc, max_context_len: int, q, out,
+                              score_scale: float, weights_in, weights_out, decay: float = 1.0, stream=None) -> None:
+        """llh_paged_prefill_weights: the same for each sequence's last rows (at most WEIGHTS_MAX_CHUNK)."""
+        self._check_weights(weights_in, weights_out)
+        self.check(self.lib.llh_paged_prefill_weights(
+            self.handle, pool.handle, ctypes.byref(desc), max_context_len, _ptr(q), _ptr(out), score_scale,
+            _ptr(weights_in), _ptr(weights_out), weights_out.shape[-1], decay, _stream(stream)))
+
+    @staticmethod
+    def _check_weights(weights_in, weights_out) -> None:
+        import torch
+
+        for w in (weights_in, weights_out):
+            if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or w.shape != weights_out.shape):
+                raise LlhError(ERR_INVALID_SHAPE, "weights are contiguous f32 of one shape")
+
+    def weights_workspace_bytes(self, num_seqs: int, max_chunk_len: int, num_q_heads: int, head_dim: int,
+                                max_context_len: int) -> int:
+        return self.lib.llh_weights_workspace_bytes(num_seqs, max_chunk_len, num_q_heads, head_dim, max_context_len)
+
+    @staticmethod
+    def select_desc(seq_lens, kv_heads: int, max_seq_len: int, budget: int, sinks: int, recent: int,
+                    weights_stride: int, keep_stride: int) -> KvSelectDesc:
+        """Descriptor of llh_kv_select over an int32 device tensor of lengths (kept alive)."""
+        d = KvSelectDesc(num_seqs=seq_lens.shape[0], kv_heads=kv_heads, max_seq_len=max_seq_len, budget=budget,
+                         sinks=sinks, recent=recent, weights_stride=weights_stride, keep_stride=keep_stride,
+                         d_seq_lens=_ptr(seq_lens))
+        d._keep = (seq_lens,)
+        return d
+
+    def kv_select(self, desc: KvSelectDesc, weights, keep, kept_lens, stream=None) -> None:
+        """llh_kv_select: the positions each (sequence, kv head) keeps, ascending, and the lengths that leaves."""
+        self.check(self.lib.llh_kv_select(self.handle, ctypes.byref(desc), _ptr(weights), _ptr(keep),
+                                          _ptr(kept_lens), _stream(stream)))
+
+    @staticmethod
+    def compact_desc(seq_lens, kept_lens, keep, src_tables, dst_tables, max_kept: int, weights_in=None,
+                     weights_out=None) -> KvCompactDesc:
+        """Descriptor of llh_kv_compact over device tensors (kept alive): keep int32 [num_seqs][kv_heads][stride],
+        tables int32 [num_seqs][blocks], weights f32 [num_seqs][kv_heads][stride] or None."""
+        d = KvCompactDesc(
+            num_seqs=seq_lens.shape[0],
+            max_kept=max_kept,
+            src_max_blocks=src_tables.shape[1],
+            dst_max_blocks=dst_tables.shape[1],
+            keep_stride=keep.shape[-1],
+            weights_in_stride=0 if weights_in is None else weights_in.shape[-1],
+            weights_out_stride=0 if weights_out is None else weights_out.shape[-1],
+            d_seq_lens=_ptr(seq_lens),
+            d_kept_lens=_ptr(kept_lens),
+            d_keep=_ptr(keep),
+            d_src_tables=_ptr(src_tables),
+            d_dst_tables=_ptr(dst_tables),
+            d_weights_in=_ptr(weights_in),
+            d_weights_out=_ptr(weights_out),
+        )
+        d._keep = (seq_lens, kept_lens, keep, src_tables, dst_tables, weights_in, weights_out)
+        return d
+
+    def kv_compact(self, pool: "KvPool", desc: KvCompactDesc, stream=None) -> None:
+        """llh_kv_compact: the kept tokens (and their weights) to the destination tables' blocks."""
+        self.check(self.lib.llh_kv_compact(self.handle, pool.handle, ctypes.byref(desc), _stream(stream)))
 
     def write_blocks(self, pool: "KvPool", blocks, k, v, stream=None) -> None:
         self.check(
