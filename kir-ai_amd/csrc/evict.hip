@@ -220,9 +220,18 @@ __global__ __launch_bounds__(D * (is16(FMT) ? 2 : 1)) void kv_compact_kernel(con
   constexpr int FLIGHT = 8;
   constexpr bool FP8 = FMT == kFp8;
   typedef typename std::conditional<ES == 2, uint16_t, uint8_t>::type elem_t;
-  const int j = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  // neighbouring destination blocks share a source block: give each XCD (workgroups go round them) a run
+  const int nx = gridDim.x, xcd = blockIdx.x % 8;
+  const int j = xcd * (nx / 8) + min(xcd, nx % 8) + (int)blockIdx.x / 8;
+  const int h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
   const int Hkv = a.pool.kv_heads;
+  // lane t (mod 16): token t of the block; its position is loaded beside the lengths (the row holds
+  // max_kept entries whatever the length is)
+  const int mine = j * BT + (lane & 15);
+  const size_t row = (size_t)b * Hkv + h;
+  const int pos = a.keep[row * a.keep_stride + min(mine, a.max_kept - 1)];
+  const int dst = a.dst_tables[(size_t)b * a.dst_max_blocks + j];
   const int kept = a.kept_lens[b];
   if (kept > a.max_kept) {
     if (tid == 0 && j == 0 && h == 0) atomicOr(a.err, kErrTooManySplits);
@@ -231,11 +240,8 @@ __global__ __launch_bounds__(D * (is16(FMT) ? 2 : 1)) void kv_compact_kernel(con
   if (j * BT >= kept) return;
   int64_t limit = min((int64_t)a.seq_lens[b], (int64_t)a.src_max_blocks * BT);
   if (a.w_in) limit = min(limit, a.w_in_stride);
-  const int dst = a.dst_tables[(size_t)b * a.dst_max_blocks + j];
-  // lane t (mod 16): token t's source block (-1: none) and offset
-  const int mine = j * BT + (lane & 15);
-  const size_t row = (size_t)b * Hkv + h;
-  const int p = mine < kept ? a.keep[row * a.keep_stride + mine] : -1;
+  // its source block (-1: none) and offset
+  const int p = mine < kept ? pos : -1;
   const bool inside = p >= 0 && p < limit;
   int blk = inside ? a.src_tables[(size_t)b * a.src_max_blocks + p / BT] : -1;
   if (blk < 0 || blk >= a.pool.n_blocks) blk = -1;
