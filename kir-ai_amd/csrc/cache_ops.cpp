@@ -121,12 +121,13 @@ int llh_kv_select(llh_ctx *ctx, const llh_kv_select_desc *desc, const float *d_w
   if (!ctx || !desc) return LLH_ERR_NULL;
   if (desc->num_seqs < 0 || desc->num_seqs > 65535)
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "num_seqs must be 0 .. 65535");
-  if (desc->kv_heads <= 0) return ctx->fail(LLH_ERR_INVALID_SHAPE, "kv_heads must be positive");
+  if (desc->kv_heads <= 0 || desc->kv_heads > 65535)
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "kv_heads must be 1 .. 65535");
   if (desc->budget <= 0 || desc->sinks < 0 || desc->recent < 0 ||
       (int64_t)desc->sinks + desc->recent > desc->budget)
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "budget must be positive and hold the sinks and the recent tokens");
-  if (desc->max_seq_len < 0 || desc->weights_stride < desc->max_seq_len)
-    return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_seq_len must be >= 0 and at most weights_stride");
+  if (desc->max_seq_len < 0 || desc->max_seq_len > kSelectMaxLen || desc->weights_stride < desc->max_seq_len)
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_seq_len must be 0 .. 2^30 and at most weights_stride");
   if (desc->keep_stride < std::min(desc->budget, desc->max_seq_len))
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "keep_stride must hold the kept positions");
   if (desc->num_seqs == 0) return LLH_OK;
@@ -151,6 +152,13 @@ int llh_kv_select(llh_ctx *ctx, const llh_kv_select_desc *desc, const float *d_w
   a.budget = desc->budget;
   a.sinks = desc->sinks;
   a.recent = desc->recent;
+  WsLease lease;
+  const size_t bytes = select_scratch_bytes(a.num_seqs, a.kv_heads, a.max_seq_len);
+  if (bytes) {
+    const int st = lease.acquire(ctx, s, bytes);
+    if (st != LLH_OK) return st;
+    a.scratch = lease.base();
+  }
   const hipError_t e = launch_kv_select(a, s);
   if (e != hipSuccess) return ctx->hip_fail(e, "selection launch");
   return LLH_OK;

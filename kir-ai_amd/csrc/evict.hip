@@ -15,11 +15,37 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / 64;
+// ---------------------------------------------------------------------------
+// selection
+// ---------------------------------------------------------------------------
+//
+// The k-th largest key is found by its digits of 11, 11 and 10 bits from the top: a histogram of
+// the next digit over the keys that share the digits so far, and the bin in which the sum from
+// the largest digit down passes k.  Eleven bits are the sign, the exponent and two bits of the
+// fraction, which spreads weights over tens of bins.  The kept positions are then those of larger
+// keys and the first of the equal ones, written in order by ballots.
+//
+// A wavefront holds 64 KPT neighbouring positions, position i * 64 + lane of them in register i:
+// loads are whole whatever the rows' alignment, and order is wavefront, register, lane.
+constexpr int kBins = 2048;
+constexpr int kSelectMaxKpt = 32;  // keys a thread holds of a row that one workgroup selects from
 
-// Exclusive sum of `v` over the threads of the workgroup; *total receives the sum of all.
-__device__ __forceinline__ int block_exclusive(int v, int *s_waves, int *total) {
+struct RowRange {
+  int len, lo, hi;  // tokens; the positions to choose from
+  int want;         // how many of those are kept
+};
+__device__ __forceinline__ RowRange row_range(const SelectArgs &a, int b) {
+  const int len = a.seq_lens[b];
+  return {len, a.sinks, len - a.recent, a.budget - a.sinks - a.recent};
+}
+// A row that needs no choice: none of it, or all.
+__device__ __forceinline__ bool row_is_plain(const SelectArgs &a, int len) {
+  return len < 0 || len > a.max_seq_len || len <= a.budget;
+}
+
+// Exclusive sum of v over the threads; s_waves: one int a wavefront.
+template <int WAVES>
+__device__ __forceinline__ int block_exclusive(int v, int *s_waves) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
 #pragma unroll
@@ -27,92 +53,337 @@ __device__ __forceinline__ int block_exclusive(int v, int *s_waves, int *total) 
     const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
-  __syncthreads();  // s_waves may still be read
   if (lane == 63) s_waves[wave] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  int before = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; w++) {
-    if (w < wave) before += s_waves[w];
-    all += s_waves[w];
-  }
-  *total = all;
+  for (int w = 0; w < WAVES; w++) before += w < wave ? s_waves[w] : 0;
   return before + x - v;
 }
 
-// One workgroup per (sequence, kv head).  The k-th largest key of the positions between the sinks
-// and the recent ones is found eight bits at a time; the kept positions are then written in order.
-__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const SelectArgs a) {
-  const int b = blockIdx.y, h = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int len = a.seq_lens[b];
-  if (len < 0 || len > a.max_seq_len) {
-    if (tid == 0 && h == 0) {
-      atomicOr(a.err, kErrTooManySplits);
-      a.kept_lens[b] = 0;
-    }
-    return;
-  }
-  if (tid == 0 && h == 0) a.kept_lens[b] = min(len, a.budget);
-  int32_t *keep = a.keep + ((size_t)b * a.kv_heads + h) * a.keep_stride;
-  if (len <= a.budget) {
-    for (int i = tid; i < len; i += kSelectThreads) keep[i] = i;
-    return;
-  }
-  const float *w = a.weights + ((size_t)b * a.kv_heads + h) * a.weights_stride;
-  const int lo = a.sinks, hi = len - a.recent;  // the positions to choose from; lo <= hi as len > budget
-  int want = a.budget - a.sinks - a.recent;
-  __shared__ int hist[256];
-  __shared__ int s_waves[kSelectWaves];
-  __shared__ int s_bin, s_above;
-  uint32_t prefix = 0, mask = 0;
-  int equal_wanted = 0;
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int p = lo + tid; p < hi; p += kSelectThreads) {
-        const uint32_t k = order_key(w[p]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+// Adds the lanes' digits to a histogram: the first lane's digit once for all lanes that share it
+// (most weights may be equal), the others one by one.
+__device__ __forceinline__ void count_digit(int *hist, int digit, bool on, int lane) {
+  const uint64_t live = __ballot(on);
+  if (!live) return;
+  const int head = __builtin_amdgcn_readlane(digit, __builtin_ctzll(live));
+  const uint64_t same = __ballot(on && digit == head);
+  if (lane == __builtin_ctzll(live)) atomicAdd(&hist[head], __builtin_popcountll(same));
+  if (on && digit != head) atomicAdd(&hist[digit], 1);
+}
+
+// The digit in which the sum of counts from the largest digit down reaches `want`, given each
+// thread's counts of its 2048 / THREADS neighbouring bins, largest first from thread 0's; *want
+// loses what the larger digits hold.  Ends with a barrier.
+template <int THREADS, int PER>
+__device__ __forceinline__ int find_digit(const int (&c)[PER], int top, int *want, int *s_waves, int *s_found) {
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) sum += c[i];
+  int above = block_exclusive<THREADS / 64>(sum, s_waves);
+  if (above < *want && above + sum >= *want) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      if (above < *want && above + c[i] >= *want) {
+        s_found[0] = top - (int)threadIdx.x * PER - i;
+        s_found[1] = above;
       }
-      __syncthreads();
-      // the bin that holds the want-th largest: sums from the top down
-      int total;
-      const int mine = tid < 256 ? hist[255 - tid] : 0;
-      const int above = block_exclusive(mine, s_waves, &total);
-      if (tid < 256 && above < want && above + mine >= want) {
-        s_bin = 255 - tid;
-        s_above = above;
-      }
-      __syncthreads();
-      prefix |= (uint32_t)s_bin << shift;
-      mask |= 255u << shift;
-      want -= s_above;
-      __syncthreads();
+      above += c[i];
     }
-    equal_wanted = want;
-  } else {
-    prefix = 0xffffffffu;  // nothing of the middle (no key reaches it: a NaN's is 0)
   }
-  int n_out = 0, n_equal = 0;
-  for (int p0 = 0; p0 < len; p0 += kSelectThreads) {
-    const int p = p0 + tid;
-    bool on = p < len && (p < lo || p >= hi);
-    bool eq = false;
-    if (p >= lo && p < hi) {
-      const uint32_t k = order_key(w[p]);
-      on = k > prefix;
-      eq = k == prefix;
-    }
-    int total;
-    const int rank = n_equal + block_exclusive(eq ? 1 : 0, s_waves, &total);
-    n_equal += total;
-    on = on || (eq && rank < equal_wanted);
-    const int at = n_out + block_exclusive(on ? 1 : 0, s_waves, &total);
-    n_out += total;
-    if (on) keep[at] = p;
+  __syncthreads();
+  *want -= s_found[1];
+  return s_found[0];
+}
+
+// Bits of digit `pass` (0, 1, 2) and where it starts.
+constexpr int kDigitShift[3] = {21, 10, 0};
+constexpr uint32_t kDigitMask[3] = {2047u, 2047u, 1023u};
+
+// Writes the kept ones of this workgroup's positions from p0 on, in order.  threshold: the least key
+// kept; of the equal ones the first `equal_wanted` in the row.  n_out, n_equal: kept and
+// equal positions of the row before p0.
+template <int THREADS, int KPT>
+__device__ __forceinline__ void write_kept(const uint32_t (&key)[KPT], const RowRange &r, int p0, uint32_t threshold,
+                                           int equal_wanted, int n_out, int n_equal, int32_t *keep, int *s_waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t below = (1ull << lane) - 1;
+  const int first = p0 + wave * 64 * KPT + lane;
+  // equal keys of the wavefronts before this one
+  int eq = 0;
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    const int p = first + 64 * i;
+    eq += __builtin_popcountll(__ballot(p >= r.lo && p < r.hi && key[i] == threshold));
+  }
+  __syncthreads();
+  if (lane == 0) s_waves[wave] = eq;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; w++) n_equal += w < wave ? s_waves[w] : 0;
+  uint32_t on = 0;  // bit i: register i is kept
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    const int p = first + 64 * i;
+    const bool mid = p >= r.lo && p < r.hi;
+    const uint64_t e = __ballot(mid && key[i] == threshold);
+    const bool k = p < r.len && (!mid || key[i] > threshold ||
+                                 (key[i] == threshold && n_equal + __builtin_popcountll(e & below) < equal_wanted));
+    n_equal += __builtin_popcountll(e);
+    count += __builtin_popcountll(__ballot(k));
+    on |= k ? 1u << i : 0u;
+  }
+  __syncthreads();
+  if (lane == 0) s_waves[wave] = count;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; w++) n_out += w < wave ? s_waves[w] : 0;
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    const bool k = on >> i & 1;
+    const uint64_t m = __ballot(k);
+    if (k) keep[n_out + __builtin_popcountll(m & below)] = first + 64 * i;
+    n_out += __builtin_popcountll(m);
   }
 }
+
+template <int THREADS, int KPT>
+__device__ __forceinline__ void load_keys(uint32_t (&key)[KPT], const float *w, const RowRange &r, int p0) {
+  const int first = p0 + (threadIdx.x >> 6) * 64 * KPT + (threadIdx.x & 63);
+  float x[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; i++) {
+    const int p = first + 64 * i;
+    x[i] = p >= r.lo && p < r.hi ? w[p] : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < KPT; i++) key[i] = order_key(x[i]);
+}
+
+// What a row's first workgroup says of it: its kept length, and a length that is out of range.
+__device__ __forceinline__ void row_lengths(const SelectArgs &a, int b, int len) {
+  const bool bad = len < 0 || len > a.max_seq_len;
+  if (bad) atomicOr(a.err, kErrTooManySplits);
+  a.kept_lens[b] = bad ? 0 : min(len, a.budget);
+}
+
+// One workgroup per (sequence, kv head), which holds the row's keys in registers.
+template <int THREADS, int KPT>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(const SelectArgs a) {
+  constexpr int PER = kBins / THREADS;
+  const int b = blockIdx.y, h = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const RowRange r = row_range(a, b);
+  if (tid == 0 && h == 0) row_lengths(a, b, r.len);
+  const size_t row = (size_t)b * a.kv_heads + h;
+  int32_t *keep = a.keep + row * a.keep_stride;
+  if (row_is_plain(a, r.len)) {
+    if (r.len <= a.max_seq_len)
+      for (int i = tid; i < r.len; i += THREADS) keep[i] = i;
+    return;
+  }
+  __shared__ int hist[kBins];
+  __shared__ int s_waves[THREADS / 64];
+  __shared__ int s_found[2];
+  uint32_t key[KPT];
+  load_keys<THREADS, KPT>(key, a.weights + row * a.weights_stride, r, 0);
+  const int first = (tid >> 6) * 64 * KPT + lane;
+  uint32_t threshold = 0xffffffffu;  // nothing of the middle: no key reaches it
+  int want = r.want;
+  if (want > 0) {
+    uint32_t prefix = 0, mask = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+#pragma unroll
+      for (int i = 0; i < PER; i++) hist[tid + i * THREADS] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KPT; i++) {
+        const int p = first + 64 * i;
+        count_digit(hist, (int)((key[i] >> kDigitShift[pass]) & kDigitMask[pass]),
+                    p >= r.lo && p < r.hi && (key[i] & mask) == prefix, lane);
+      }
+      __syncthreads();
+      int c[PER];
+#pragma unroll
+      for (int i = 0; i < PER; i++) c[i] = hist[kBins - 1 - tid * PER - i];
+      const int digit = find_digit<THREADS, PER>(c, kBins - 1, &want, s_waves, s_found);
+      prefix |= (uint32_t)digit << kDigitShift[pass];
+      mask |= kDigitMask[pass] << kDigitShift[pass];
+    }
+    threshold = prefix;
+  }
+  write_kept<THREADS, KPT>(key, r, 0, threshold, want, 0, 0, keep, s_waves);
+}
+
+// Longer rows: tiles of kTileKeys positions, a launch per digit and one that writes.  Every tile
+// leaves its histogram (16-bit counts, two a word) in the workspace, and every workgroup of the
+// next launch adds up the row's: no counter has to be cleared, and nothing depends on order.
+constexpr int kTileThreads = 1024;
+constexpr int kTileKpt = 8;
+constexpr int kTileKeys = kTileThreads * kTileKpt;
+constexpr int kTileWords = kBins / 2;
+struct TileState {
+  int digit[2], want[2];  // after the first and the second digit
+};
+struct TileView {
+  uint32_t *hist;    // [rows][tiles][3][kTileWords]
+  int *larger;       // [rows][tiles][2]: keys of the tile larger by the first / second digit
+  TileState *state;  // [rows]
+};
+__host__ __device__ inline size_t tile_bytes(size_t rows, size_t tiles) {
+  return rows * tiles * (3 * kTileWords + 2) * 4 + rows * sizeof(TileState);
+}
+__host__ __device__ inline TileView tile_view(void *ws, size_t rows, size_t tiles) {
+  TileView v;
+  v.hist = static_cast<uint32_t *>(ws);
+  v.larger = reinterpret_cast<int *>(v.hist + rows * tiles * 3 * kTileWords);
+  v.state = reinterpret_cast<TileState *>(v.larger + rows * tiles * 2);
+  return v;
+}
+
+// This thread's two bins of the row's histogram of one digit, the larger first.
+__device__ __forceinline__ void row_counts(const uint32_t *hist, int tiles, int (&c)[2]) {
+  c[0] = c[1] = 0;
+  const uint32_t *p = hist + (kTileWords - 1 - threadIdx.x);
+#pragma unroll 8
+  for (int t = 0; t < tiles; t++) {
+    const uint32_t w = p[(size_t)t * 3 * kTileWords];
+    c[0] += (int)(w >> 16);
+    c[1] += (int)(w & 0xffffu);
+  }
+}
+
+// PASS 0, 1, 2: the histogram of that digit; 3: the positions.
+template <int PASS>
+__global__ __launch_bounds__(kTileThreads) void kv_select_tile_kernel(const SelectArgs a) {
+  const int tile = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const RowRange r = row_range(a, b);
+  const size_t row = (size_t)b * a.kv_heads + h;
+  int32_t *keep = a.keep + row * a.keep_stride;
+  if (PASS == 3 && tid == 0 && h == 0 && tile == 0) row_lengths(a, b, r.len);
+  const int p0 = tile * kTileKeys;
+  if (row_is_plain(a, r.len)) {
+    if (PASS == 3 && r.len <= a.max_seq_len)
+      for (int i = p0 + tid; i < min(r.len, p0 + kTileKeys); i += kTileThreads) keep[i] = i;
+    return;
+  }
+  if (p0 >= r.len) return;
+  const int tiles = (r.len + kTileKeys - 1) / kTileKeys;
+  const TileView v = tile_view(a.scratch, (size_t)a.num_seqs * a.kv_heads, gridDim.x);
+  uint32_t *const hist_row = v.hist + row * gridDim.x * 3 * kTileWords;
+  __shared__ int hist[kBins];
+  __shared__ int s_waves[kTileThreads / 64];
+  __shared__ int s_found[2];
+  __shared__ int s_before[2][kTileThreads / 64];
+  uint32_t key[kTileKpt];
+  load_keys<kTileThreads, kTileKpt>(key, a.weights + row * a.weights_stride, r, p0);
+  const int first = p0 + wave * 64 * kTileKpt + lane;
+
+  // the digits so far
+  uint32_t prefix = 0, mask = 0;
+  int want = r.want;
+  if (want > 0) {
+    if (PASS >= 2) {
+      const TileState s = v.state[row];
+      prefix = (uint32_t)s.digit[0] << kDigitShift[0];
+      mask = kDigitMask[0] << kDigitShift[0];
+      want = s.want[0];
+      if (PASS == 3) {
+        prefix |= (uint32_t)s.digit[1] << kDigitShift[1];
+        mask |= kDigitMask[1] << kDigitShift[1];
+        want = s.want[1];
+      }
+    }
+    if (PASS >= 1) {
+      int c[2];
+      row_counts(hist_row + (PASS - 1) * kTileWords, tiles, c);
+      const int digit = find_digit<kTileThreads, 2>(c, kBins - 1, &want, s_waves, s_found);
+      const uint32_t old_prefix = prefix, old_mask = mask;
+      prefix |= (uint32_t)digit << kDigitShift[PASS - 1];
+      mask |= kDigitMask[PASS - 1] << kDigitShift[PASS - 1];
+      if (PASS < 3) {
+        if (tile == 0 && tid == 0) {
+          v.state[row].digit[PASS - 1] = digit;
+          v.state[row].want[PASS - 1] = want;
+        }
+        // keys that are larger by this digit
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kTileKpt; i++) {
+          const int p = first + 64 * i;
+          n += __builtin_popcountll(
+              __ballot(p >= r.lo && p < r.hi && (key[i] & old_mask) == old_prefix && (key[i] & mask) > prefix));
+        }
+        if (lane == 0) s_before[0][wave] = n;
+        __syncthreads();
+        if (tid == 0) {
+          int all = 0;
+          for (int w = 0; w < kTileThreads / 64; w++) all += s_before[0][w];
+          v.larger[(row * gridDim.x + tile) * 2 + PASS - 1] = all;
+        }
+      }
+    }
+    if (PASS < 3) {
+      for (int i = tid; i < kBins; i += kTileThreads) hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kTileKpt; i++) {
+        const int p = first + 64 * i;
+        count_digit(hist, (int)((key[i] >> kDigitShift[PASS % 3]) & kDigitMask[PASS % 3]),
+                    p >= r.lo && p < r.hi && (key[i] & mask) == prefix, lane);
+      }
+      __syncthreads();
+      hist_row[((size_t)tile * 3 + PASS) * kTileWords + tid] = (uint32_t)hist[2 * tid] | ((uint32_t)hist[2 * tid + 1] << 16);
+    }
+  } else {
+    prefix = 0xffffffffu;  // nothing of the middle: no key reaches it
+  }
+  if (PASS < 3) return;
+
+  // kept and equal positions of the tiles before this one, a tile per wavefront
+  int larger = 0, equal = 0;
+  if (r.want > 0) {
+    const int digit = (int)(prefix & kDigitMask[2]);
+    for (int t = wave; t < tile; t += kTileThreads / 64) {
+      const uint32_t *ht = hist_row + ((size_t)t * 3 + 2) * kTileWords;
+      if (lane == 0) {
+        const int *l = &v.larger[(row * gridDim.x + t) * 2];
+        larger += l[0] + l[1];
+      }
+      for (int i = lane; i < 1024 / 2; i += 64) {  // the last digit has ten bits
+        const uint32_t w = ht[i];
+        const int lo_bin = 2 * i, hi_bin = 2 * i + 1;
+        larger += (lo_bin > digit ? (int)(w & 0xffffu) : 0) + (hi_bin > digit ? (int)(w >> 16) : 0);
+        equal += (lo_bin == digit ? (int)(w & 0xffffu) : 0) + (hi_bin == digit ? (int)(w >> 16) : 0);
+      }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      larger += __shfl_xor(larger, d);
+      equal += __shfl_xor(equal, d);
+    }
+  }
+  if (lane == 0) {
+    s_before[0][wave] = larger;
+    s_before[1][wave] = equal;
+  }
+  __syncthreads();
+  int n_larger = 0, n_equal = 0;
+#pragma unroll
+  for (int w = 0; w < kTileThreads / 64; w++) {
+    n_larger += s_before[0][w];
+    n_equal += s_before[1][w];
+  }
+  const int n_out = min(p0, r.lo) + max(0, p0 - r.hi) + n_larger + min(n_equal, want);
+  write_kept<kTileThreads, kTileKpt>(key, r, p0, prefix, want, n_out, n_equal, keep, s_waves);
+}
+
+// ---------------------------------------------------------------------------
+// compaction
+// ---------------------------------------------------------------------------
 
 // One workgroup per (destination block, kv head, sequence), element by element: any block size,
 // head_dim and format but int8 rows.
@@ -400,9 +671,28 @@ void launch_compact_d(const CompactArgs &a, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
+size_t select_scratch_bytes(int num_seqs, int kv_heads, int max_seq_len) {
+  if (max_seq_len <= 1024 * kSelectMaxKpt) return 0;
+  return tile_bytes((size_t)num_seqs * kv_heads, (max_seq_len + kTileKeys - 1) / kTileKeys);
+}
+
 hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s) {
   if (a.num_seqs <= 0) return hipSuccess;
-  hipLaunchKernelGGL(kv_select_kernel, dim3(a.kv_heads, a.num_seqs), dim3(kSelectThreads), 0, s, a);
+  const int n = a.max_seq_len;
+  const dim3 grid(a.kv_heads, a.num_seqs);
+  if (n <= 1024 * kSelectMaxKpt) {
+    if (n <= 1024) hipLaunchKernelGGL((kv_select_kernel<256, 4>), grid, dim3(256), 0, s, a);
+    else if (n <= 4096) hipLaunchKernelGGL((kv_select_kernel<1024, 4>), grid, dim3(1024), 0, s, a);
+    else if (n <= 8192) hipLaunchKernelGGL((kv_select_kernel<1024, 8>), grid, dim3(1024), 0, s, a);
+    else if (n <= 16384) hipLaunchKernelGGL((kv_select_kernel<1024, 16>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((kv_select_kernel<1024, kSelectMaxKpt>), grid, dim3(1024), 0, s, a);
+    return hipGetLastError();
+  }
+  const dim3 tiles((n + kTileKeys - 1) / kTileKeys, a.kv_heads, a.num_seqs);
+  hipLaunchKernelGGL(kv_select_tile_kernel<0>, tiles, dim3(kTileThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_select_tile_kernel<1>, tiles, dim3(kTileThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_select_tile_kernel<2>, tiles, dim3(kTileThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_select_tile_kernel<3>, tiles, dim3(kTileThreads), 0, s, a);
   return hipGetLastError();
 }
 

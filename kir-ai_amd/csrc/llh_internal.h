@@ -221,7 +221,11 @@ struct SelectArgs {
   int64_t weights_stride, keep_stride;
   int32_t *err;
   int32_t num_seqs, kv_heads, max_seq_len, budget, sinks, recent;
+  void *scratch;            // select_scratch_bytes
 };
+constexpr int kSelectMaxLen = 1 << 30;
+// bytes of SelectArgs::scratch: 0 where one workgroup holds a row
+size_t select_scratch_bytes(int num_seqs, int kv_heads, int max_seq_len);
 
 struct CompactArgs {
   PoolView pool;

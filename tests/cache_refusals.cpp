@@ -187,6 +187,11 @@ static void select_cases() {
   select_case("negative sequences", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.num_seqs = -1; });
   select_case("too many sequences", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.num_seqs = 65536; });
   select_case("no heads", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.kv_heads = 0; });
+  select_case("too many heads", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.kv_heads = 65536; });
+  select_case("length past the bound", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) {
+    d.max_seq_len = (1 << 30) + 1;
+    d.weights_stride = d.max_seq_len;
+  });
   select_case("no budget", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.budget = d.sinks = d.recent = 0; });
   select_case("negative sinks", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.sinks = -1; });
   select_case("negative recent", LLH_ERR_INVALID_SHAPE, [](D &d, W &, K &, K &) { d.recent = -1; });
