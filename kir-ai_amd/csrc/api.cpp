@@ -1356,6 +1356,7 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   if (!d_q || !d_out || !d_w || !c.lens || !c.tables)
     return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
   if (c.num_seqs > 65535) return ctx->fail(LLH_ERR_INVALID_SHAPE, "num_seqs must be <= 65535");
+  if (c.max_ctx > kWeightsMaxLen) return ctx->fail(LLH_ERR_INVALID_SHAPE, "context too long for one call");
   if (stride < std::max(1, c.max_ctx))
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "weights_stride must hold the longest context");
   if ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 1)
@@ -1385,10 +1386,14 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
         c.total_hint > 0 ? tiles * ((long long)c.total_hint / uk + c.num_seqs) : tiles * units * c.num_seqs;
     sr = split_rows(ctx, pv, tiles * c.num_seqs, units, total, rows, SIZE_MAX);
   }
-  const size_t ml_off = sr.bytes;
-  const size_t sc_off = ml_off + align_up(rows * sizeof(float2));
+  else {
+    sr.max_splits = 1;
+    sr.single_units = INT32_MAX / 2;
+  }
+  // partial outputs, the (max, sum) pairs of every split, the scores
+  const size_t ml_off = sr.max_splits > 1 ? align_up(rows * sr.max_splits * pv.head_dim * sizeof(float)) : 0;
+  const size_t sc_off = ml_off + align_up(rows * sr.max_splits * sizeof(float2));
   const int64_t sc_stride = score_stride(span);
-  if (sc_stride > INT32_MAX) return ctx->fail(LLH_ERR_INVALID_SHAPE, "context too long for one call");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   WsLease lease;
   const int st = lease.acquire(ctx, s, sc_off + rows * sc_stride * sizeof(float));
@@ -1401,8 +1406,8 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   r.chunk_starts = c.chunk_starts;
   r.context_lens = c.lens;
   r.tables = c.tables;
-  r.ws_ml = reinterpret_cast<float2 *>(lease.base());
-  r.ws_o = reinterpret_cast<float *>(lease.base() + sr.o_off);
+  r.ws_o = reinterpret_cast<float *>(lease.base());
+  r.ws_ml = reinterpret_cast<float2 *>(lease.base() + ml_off);
   r.err = lease.err();
   r.num_seqs = c.num_seqs;
   r.max_rows = c.max_rows;
@@ -1410,7 +1415,7 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   r.max_blocks = c.max_blocks;
   r.window = c.window;
   r.split_units = std::max(1, sr.split_units);
-  r.max_splits = std::max(1, sr.max_splits);
+  r.max_splits = sr.max_splits;
   r.single_units = sr.single_units;
   r.max_span = (int32_t)span;
   r.max_len = std::max(1, c.max_ctx);
@@ -1418,7 +1423,6 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   r.scale = score_scale;
   r.scale_log2e = score_scale * 1.4426950408889634f;
   r.gate = static_cast<const uint16_t *>(c.gate);
-  r.row_ml = reinterpret_cast<float2 *>(lease.base() + ml_off);
   r.scores = reinterpret_cast<float *>(lease.base() + sc_off);
   r.score_stride = (int32_t)sc_stride;
   w.w_in = d_in;
@@ -1429,7 +1433,7 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   if (tuned) ctx->routes[c.chunk_starts ? LLH_ROUTE_ROWS_PREFILL : LLH_ROUTE_ROWS_DECODE]++;
   else (c.chunk_starts ? ctx->generic_prefill_calls : ctx->generic_decode_calls)++;
   hipError_t e = tuned ? launch_rows(r, false, s) : launch_weights_generic(r, s);
-  if (e == hipSuccess) e = launch_weights_accumulate(w, c.max_ctx, s);
+  if (e == hipSuccess) e = launch_weights_finish(w, c.max_ctx, s);
   if (e != hipSuccess) return ctx->hip_fail(e, "attention weights launch");
   return LLH_OK;
 }
@@ -1444,8 +1448,8 @@ size_t llh_weights_workspace_bytes(int32_t num_seqs, int32_t max_chunk_len, int3
   const size_t rows = (size_t)num_seqs * max_chunk_len * num_q_heads;
   // split_rows: at most four splits a workgroup slot, 16 rows each
   const size_t partial = std::min<size_t>(rows * kRowsMaxSplits, (size_t)64 * 1024);
-  return align_up(partial * sizeof(float2)) + align_up(partial * head_dim * sizeof(float)) + kAlign +
-         align_up(rows * sizeof(float2)) + rows * score_stride(std::max(1, max_context_len)) * sizeof(float);
+  return align_up(partial * head_dim * sizeof(float)) + align_up(std::max(partial, rows) * sizeof(float2)) +
+         rows * score_stride(std::max(1, max_context_len)) * sizeof(float);
 }
 
 int llh_paged_decode_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_decode_desc *desc, const void *d_q,

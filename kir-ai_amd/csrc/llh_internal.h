@@ -178,16 +178,16 @@ struct RowsArgs {
   float scale_log2e;
   const uint16_t *gate;
   // attention weights (weights.hip): null, or [num_seqs][max_rows][Hq][score_stride] scores in
-  // log2 units, position p at p - weights_base(first attended position), and the (max, sum) of each row
+  // log2 units, position p at p - weights_base(first attended position); ws_ml then holds the pairs
+  // of sequences in one split too
   float *scores;
-  float2 *row_ml;           // [num_seqs][max_rows][Hq]
   int32_t score_stride;     // a multiple of 64
 };
 int rows_unit_keys(int head_dim);
 // Scores are stored from a multiple of 64 positions on, so that units and vectors of keys are whole.
 __host__ __device__ constexpr int weights_base(int lo) { return lo & ~63; }
 
-// Accumulation of the softmax weights over the rows of `rows` (its scores and row_ml).
+// Accumulation of the softmax weights over the rows of `rows` (its scores and ws_ml).
 struct WeightsArgs {
   RowsArgs rows;
   const float *w_in;        // [num_seqs][Hkv][stride], or null (zeros)
@@ -343,10 +343,12 @@ hipError_t launch_decode_fp8(const uint8_t *codes, float *out, int32_t n, hipStr
 // encoder differs from the integer reference rule
 hipError_t launch_fp8_encode_check(unsigned long long *mismatches, hipStream_t s);
 hipError_t launch_matvec_bf16(const MatvecArgs &a, hipStream_t s);
-// scores, row_ml and output of every shape the packed-row kernel does not take (head_dim <= 512)
+// scores, ws_ml (one split) and output of every shape the packed-row kernel does not take (head_dim <= 512)
 constexpr int kWeightsMaxDim = 512;
+constexpr int kWeightsMaxLen = 1 << 30;
 hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s);
-hipError_t launch_weights_accumulate(const WeightsArgs &a, int max_len, hipStream_t s);
+// merges the splits and accumulates
+hipError_t launch_weights_finish(const WeightsArgs &a, int max_len, hipStream_t s);
 hipError_t launch_qk_rope(const QkRopeArgs &a, hipStream_t s);
 hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s);
 hipError_t launch_kv_compact(const CompactArgs &a, hipStream_t s);

@@ -111,13 +111,6 @@ __device__ __forceinline__ void f16x8_to_bf16(const u32x4_t &w, u32x4_t &hi, u32
   }
 }
 
-// 1 / (weight sum).  No weight at all (every key masked, or every score -inf) gives the zero
-// row of the tile prefill and the reference-order decode, and the NaN (0 / 0) of the vector
-// decode kernels in the calls that are theirs too.
-__device__ __forceinline__ float row_inv(const RowsArgs &a, float ll) {
-  return ll == 0.0f && (a.chunk_starts || a.zero_bad || a.scores) ? 0.0f : 1.0f / ll;
-}
-
 // keys per unit: K and V of a unit take 64 operand registers each in 16-bit formats (32 in
 // 8-bit ones)
 template <int D>
@@ -575,7 +568,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
     if (sq.n_splits == 1) {
       const float inv = row_inv(a, ll);
       if constexpr (SCORES) {
-        if (d == 0) a.row_ml[((size_t)b * a.max_rows + tok) * a.q_heads + head] = make_float2(mm, ll);
+        if (d == 0)
+          a.ws_ml[(((size_t)b * a.max_rows + tok) * a.q_heads + head) * a.max_splits] = make_float2(mm, ll);
       }
       const size_t o = ((size_t)(sq.c0 + tok) * a.q_heads + head) * D + d;
 #pragma unroll
@@ -613,28 +607,6 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
   merge_splits<D, false>(a, sq, b, kvh, G, row0, live, 0, kSplitGroup, n_groups);
 }
 
-// Merge of the n <= N splits of one (query row, head): every partial row in flight at
-// once, the (max, sum) pairs one per lane, split weights through v_readlane.
-template <int D, int N>
-__device__ __forceinline__ void rows_merge(const RowsArgs &a, size_t prow, size_t orow, int last, int d) {
-  const size_t p0 = prow * a.max_splits;
-  float o_sp[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) o_sp[i] = a.ws_o[(p0 + min(i, last)) * D + d];
-  const int li = d & 63;
-  const float2 ml = a.ws_ml[p0 + min(li, last)];
-  const float mx[1] = {li <= last ? ml.x : -INFINITY}, ly[1] = {ml.y};
-  float f[1], top;
-  const float ll = merge_weights<1>(mx, ly, li, f, &top);
-  if (a.row_ml && d == 0) a.row_ml[prow] = make_float2(top, ll);
-  float oo = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; i++)  // nothing of the places past the last (0 x infinity is NaN)
-    oo += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[0]), i)) * (i <= last ? o_sp[i] : 0.0f);
-  const float inv = row_inv(a, ll);
-  a.out[orow * D + d] = f32_to_bf16_rne(gated(oo * inv, a.gate, orow * D + d));
-}
-
 template <int D, int UK>
 __global__ __launch_bounds__(D) void paged_rows_merge_kernel(const RowsArgs a) {
   const int b = blockIdx.y;
@@ -643,12 +615,7 @@ __global__ __launch_bounds__(D) void paged_rows_merge_kernel(const RowsArgs a) {
   if (sq.skip || tok >= sq.chunk || sq.n_splits <= 1) return;
   const size_t prow = (size_t)b * a.max_rows * a.q_heads + blockIdx.x;  // row of the partials
   const size_t orow = (size_t)sq.c0 * a.q_heads + blockIdx.x;           // and of the output
-  const int last = sq.n_splits - 1;
-  const int d = threadIdx.x;
-  if (last < 8) return rows_merge<D, 8>(a, prow, orow, last, d);
-  if (last < 16) return rows_merge<D, 16>(a, prow, orow, last, d);
-  if (last < 32) return rows_merge<D, 32>(a, prow, orow, last, d);
-  return rows_merge<D, kRowsMaxSplits>(a, prow, orow, last, d);
+  rows_merge<D>(a, prow, orow, sq.n_splits - 1, threadIdx.x);
 }
 
 template <int D, int FMT, int PARTS, bool SCORES = false>
@@ -659,7 +626,7 @@ hipError_t launch_rows_t(const RowsArgs &a, hipStream_t s, void *hu, LaunchHook 
                      dim3(64 * WAVES), 0, s, a);
   hipError_t e = hipGetLastError();
   if (hook) hook(hu, 1, s);
-  if (e != hipSuccess || a.max_splits <= 1 || a.counters) return e;
+  if (e != hipSuccess || a.max_splits <= 1 || a.counters || SCORES) return e;  // (SCORES: weights.hip merges)
   hipLaunchKernelGGL((paged_rows_merge_kernel<D, kUnitKeys<D>>), dim3(a.max_rows * a.q_heads, a.num_seqs), dim3(D), 0,
                      s, a);
   return hipGetLastError();

@@ -137,6 +137,11 @@ static void weights_cases() {
   weights_case("blocks", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.blocks = 0; });
   weights_case("window", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.window = -1; });
   weights_case("negative length", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.max_len = -1; });
+  weights_case("length past the bound", LLH_ERR_INVALID_SHAPE, [](Weights &c) {
+    c.max_len = (1 << 30) + 1;
+    c.stride = int64_t{1} << 31;
+    c.blocks = 1 << 27;
+  });
   weights_case("weights stride", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.stride = 99; });
   weights_case("empty weights", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.stride = c.max_len = 0; });
   weights_case("null queries", LLH_ERR_NULL, [](Weights &c) { c.q = nullptr; });
