@@ -43,22 +43,37 @@ __device__ __forceinline__ bool row_is_plain(const SelectArgs &a, int len) {
   return len < 0 || len > a.max_seq_len || len <= a.budget;
 }
 
-// Exclusive sum of v over the threads; s_waves: one int a wavefront.
+// Sum of v over the lanes up to this one (DPP: shifts within a row of 16, then the rows' totals).
+__device__ __forceinline__ int wave_inclusive(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: rows 2 and 3
+  return v;
+}
+
+// Sum of the wavefronts' numbers before this one's.
 template <int WAVES>
-__device__ __forceinline__ int block_exclusive(int v, int *s_waves) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) s_waves[wave] = x;
-  __syncthreads();
+__device__ __forceinline__ int waves_before(const int *s_waves, int wave) {
   int before = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; w++) before += w < wave ? s_waves[w] : 0;
-  return before + x - v;
+  for (int w = 0; w < WAVES; w += 4) {
+    const int4 x = *reinterpret_cast<const int4 *>(s_waves + w);
+    before += (w < wave ? x.x : 0) + (w + 1 < wave ? x.y : 0) + (w + 2 < wave ? x.z : 0) + (w + 3 < wave ? x.w : 0);
+  }
+  return before;
+}
+
+// Exclusive sum of v over the threads; s_waves: one int a wavefront, 16-byte aligned.
+template <int WAVES>
+__device__ __forceinline__ int block_exclusive(int v, int *s_waves) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int x = wave_inclusive(v);
+  if (lane == 63) s_waves[wave] = x;
+  __syncthreads();
+  return waves_before<WAVES>(s_waves, wave) + x - v;
 }
 
 // Adds the lanes' digits to a histogram: the first lane's digit once for all lanes that share it
@@ -74,9 +89,11 @@ __device__ __forceinline__ void count_digit(int *hist, int digit, bool on, int l
 
 // The digit in which the sum of counts from the largest digit down reaches `want`, given each
 // thread's counts of its 2048 / THREADS neighbouring bins, largest first from thread 0's; *want
-// loses what the larger digits hold.  Ends with a barrier.
+// loses what the larger digits hold, *all: whether every key of the digit is wanted.  Ends with a
+// barrier.
 template <int THREADS, int PER>
-__device__ __forceinline__ int find_digit(const int (&c)[PER], int top, int *want, int *s_waves, int *s_found) {
+__device__ __forceinline__ int find_digit(const int (&c)[PER], int top, int *want, bool *all, int *s_waves,
+                                          int *s_found) {
   int sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; i++) sum += c[i];
@@ -87,12 +104,14 @@ __device__ __forceinline__ int find_digit(const int (&c)[PER], int top, int *wan
       if (above < *want && above + c[i] >= *want) {
         s_found[0] = top - (int)threadIdx.x * PER - i;
         s_found[1] = above;
+        s_found[2] = c[i];
       }
       above += c[i];
     }
   }
   __syncthreads();
   *want -= s_found[1];
+  *all = s_found[2] == *want;
   return s_found[0];
 }
 
@@ -106,7 +125,7 @@ constexpr uint32_t kDigitMask[3] = {2047u, 2047u, 1023u};
 template <int THREADS, int KPT>
 __device__ __forceinline__ void write_kept(const uint32_t (&key)[KPT], const RowRange &r, int p0, uint32_t threshold,
                                            int equal_wanted, int n_out, int n_equal, int32_t *keep, int *s_waves) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint64_t below = (1ull << lane) - 1;
   const int first = p0 + wave * 64 * KPT + lane;
   // equal keys of the wavefronts before this one
@@ -119,8 +138,7 @@ __device__ __forceinline__ void write_kept(const uint32_t (&key)[KPT], const Row
   __syncthreads();
   if (lane == 0) s_waves[wave] = eq;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; w++) n_equal += w < wave ? s_waves[w] : 0;
+  n_equal += waves_before<THREADS / 64>(s_waves, wave);
   uint32_t on = 0;  // bit i: register i is kept
   int count = 0;
 #pragma unroll
@@ -137,8 +155,7 @@ __device__ __forceinline__ void write_kept(const uint32_t (&key)[KPT], const Row
   __syncthreads();
   if (lane == 0) s_waves[wave] = count;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; w++) n_out += w < wave ? s_waves[w] : 0;
+  n_out += waves_before<THREADS / 64>(s_waves, wave);
 #pragma unroll
   for (int i = 0; i < KPT; i++) {
     const bool k = on >> i & 1;
@@ -184,8 +201,8 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const SelectArgs a) 
     return;
   }
   __shared__ int hist[kBins];
-  __shared__ int s_waves[THREADS / 64];
-  __shared__ int s_found[2];
+  __shared__ __attribute__((aligned(16))) int s_waves[THREADS / 64];
+  __shared__ int s_found[3];
   uint32_t key[KPT];
   load_keys<THREADS, KPT>(key, a.weights + row * a.weights_stride, r, 0);
   const int first = (tid >> 6) * 64 * KPT + lane;
@@ -193,8 +210,10 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const SelectArgs a) 
   int want = r.want;
   if (want > 0) {
     uint32_t prefix = 0, mask = 0;
+    bool all = false;
 #pragma unroll
     for (int pass = 0; pass < 3; pass++) {
+      if (all) break;
 #pragma unroll
       for (int i = 0; i < PER; i++) hist[tid + i * THREADS] = 0;
       __syncthreads();
@@ -208,11 +227,15 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const SelectArgs a) 
       int c[PER];
 #pragma unroll
       for (int i = 0; i < PER; i++) c[i] = hist[kBins - 1 - tid * PER - i];
-      const int digit = find_digit<THREADS, PER>(c, kBins - 1, &want, s_waves, s_found);
+      const int digit = find_digit<THREADS, PER>(c, kBins - 1, &want, &all, s_waves, s_found);
       prefix |= (uint32_t)digit << kDigitShift[pass];
       mask |= kDigitMask[pass] << kDigitShift[pass];
     }
     threshold = prefix;
+    if (all) {  // every key from the digits so far on is kept (not every key of all: prefix > 0)
+      threshold = prefix - 1;
+      want = 0;
+    }
   }
   write_kept<THREADS, KPT>(key, r, 0, threshold, want, 0, 0, keep, s_waves);
 }
@@ -275,8 +298,8 @@ __global__ __launch_bounds__(kTileThreads) void kv_select_tile_kernel(const Sele
   const TileView v = tile_view(a.scratch, (size_t)a.num_seqs * a.kv_heads, gridDim.x);
   uint32_t *const hist_row = v.hist + row * gridDim.x * 3 * kTileWords;
   __shared__ int hist[kBins];
-  __shared__ int s_waves[kTileThreads / 64];
-  __shared__ int s_found[2];
+  __shared__ __attribute__((aligned(16))) int s_waves[kTileThreads / 64];
+  __shared__ int s_found[3];
   __shared__ int s_before[2][kTileThreads / 64];
   uint32_t key[kTileKpt];
   load_keys<kTileThreads, kTileKpt>(key, a.weights + row * a.weights_stride, r, p0);
@@ -300,7 +323,8 @@ __global__ __launch_bounds__(kTileThreads) void kv_select_tile_kernel(const Sele
     if (PASS >= 1) {
       int c[2];
       row_counts(hist_row + (PASS - 1) * kTileWords, tiles, c);
-      const int digit = find_digit<kTileThreads, 2>(c, kBins - 1, &want, s_waves, s_found);
+      bool all;
+      const int digit = find_digit<kTileThreads, 2>(c, kBins - 1, &want, &all, s_waves, s_found);
       const uint32_t old_prefix = prefix, old_mask = mask;
       prefix |= (uint32_t)digit << kDigitShift[PASS - 1];
       mask |= kDigitMask[PASS - 1] << kDigitShift[PASS - 1];

@@ -91,10 +91,320 @@ __global__ __launch_bounds__(64) void qk_rope_generic_kernel(const QkRopeArgs a)
   }
 }
 
+// head_dim 128 or 256, rows of 16-byte pieces: a row is 16 (32) lanes of 8 elements.  The groups
+// of lanes of a token share its heads out, so that a lane turns the same elements of every head and
+// computes its sines and cosines once.  Behind the workgroups of the queries' and keys' rows come
+// those that put the values into the pool (values_to_pool), in the same launch.
+//
+// PAIRS: which element turns with which.  kAdjacent: 2i and 2i + 1, in one lane; kHalves: i and
+// i + R / 2, a lane R / 16 further (R a multiple of 16), by a shuffle; kFull: the same at R = D, by DPP
+// (or a permlane swap at 256).
+enum { kAdjacent, kHalves, kFull };
+
+__device__ __forceinline__ void unpack8(const u32x4_t &w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    x[2 * i] = bf16_lo(w[i]);
+    x[2 * i + 1] = bf16_hi(w[i]);
+  }
+}
+__device__ __forceinline__ u32x4_t load8(const uint16_t *p) { return *reinterpret_cast<const u32x4_t *>(p); }
+// (outputs and values may lie anywhere: what a row's numbers are does not depend on it)
+__device__ __forceinline__ u32x4_t load8_any(const uint16_t *p, bool aligned) {
+  if (aligned) return load8(p);
+  u32x4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+  return w;
+}
+__device__ __forceinline__ void store8_any(uint16_t *p, const u32x4_t &w, bool aligned) {
+  if (aligned) {
+    *reinterpret_cast<u32x4_t *>(p) = w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    p[2 * i] = (uint16_t)w[i];
+    p[2 * i + 1] = (uint16_t)(w[i] >> 16);
+  }
+}
+__device__ __forceinline__ u32x4_t to_f16(const u32x4_t &w) {
+  u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = pack_f16(bf16_lo(w[i]), bf16_hi(w[i]));
+  return r;
+}
+
+// Block and offset of a slot (a division of 64-bit numbers takes a hundred instructions).
+__device__ __forceinline__ void split_slot(int64_t slot, int bt, int64_t &blk, int &off) {
+  if (bt == kFastBlockTokens) {
+    blk = slot >> 4;
+    off = (int)slot & 15;
+  } else {
+    blk = slot / bt;
+    off = (int)(slot % bt);
+  }
+}
+
+// Puts the values of one kv head of 16 tokens into a bf16 or fp16 pool.  V lies dim-major, 16 tokens
+// of a dim side by side, so tokens that fill a whole block are turned in LDS and written 16 bytes a
+// lane; rows of the call that fill a block need not start at a multiple of 16 of them, so a workgroup
+// takes the runs that start in its 16 rows (a run: neighbouring rows in neighbouring slots of one
+// block), wherever they end.  Runs that do not fill a block are written element by element, a
+// row per wavefront.  The 16 rows are loaded beside their slots, which only say where they go.
+template <int D>
+__device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, int h, bool aligned) {
+  constexpr int BT = kFastBlockTokens;
+  constexpr int LT = D / 8, ROUND = 256 / LT;  // lanes a row, rows a round
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i0 = tile * BT;
+  const int bt = a.pool.block_tokens;
+  const bool f16 = a.pool.format == kF16;
+  uint16_t *const v_dst = static_cast<uint16_t *>(a.v_dst);
+  const uint16_t *const src = a.v + (size_t)h * D;
+  __shared__ uint16_t lv[BT][D + 8];
+  // 16 rows from row i on (the call's last again past it) into registers, and from there to LDS as stored
+  u32x4_t w[BT / ROUND];
+  auto load_rows = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < BT / ROUND; r++)
+      w[r] = load8_any(src + min(i + r * ROUND + tid / LT, a.n - 1) * a.v_stride + 8 * (tid % LT), aligned);
+  };
+  auto rows_to_lds = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < BT / ROUND; r++)
+      *reinterpret_cast<u32x4_t *>(&lv[r * ROUND + tid / LT][8 * (tid % LT)]) = f16 ? to_f16(w[r]) : w[r];
+    __syncthreads();
+  };
+  load_rows(i0);
+  // lane l: the slot of row i0 - 1 + l
+  const int i = i0 - 1 + lane;
+  const int64_t slot = lane <= 32 && i >= 0 && i < a.n ? a.slots[i] : -1;
+  int64_t blk;
+  int off;
+  split_slot(slot, bt, blk, off);
+  const bool valid = slot >= 0 && blk < a.pool.n_blocks;
+  const int64_t prev = __shfl_up(slot, 1);
+  const bool prev_valid = __shfl_up((int)valid, 1) != 0;
+  // (other block sizes have no runs)
+  const bool start = bt != BT || !(lane > 0 && prev_valid && slot == prev + 1) || off == 0;
+  if (tid >= 1 && tid <= BT && i < a.n && !valid && h == 0) atomicOr(a.err, kErrBadBlock);
+  const uint64_t starts = __ballot(valid && start && lane >= 1 && lane <= BT);
+  const uint64_t conts = __ballot(valid && !start);
+  auto slot_of = [&](int l) __attribute__((always_inline)) {
+    return ((int64_t)__builtin_amdgcn_readlane((int)(slot >> 32), l) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)slot, l);
+  };
+  rows_to_lds();
+
+  // runs that do not fill a block: this workgroup's own rows from LDS, further ones from memory
+  uint64_t whole = 0, loose = 0;
+  for (uint64_t m = starts; m; m &= m - 1) {
+    const int l0 = __builtin_ctzll(m);
+    const int len = 1 + __builtin_ctzll(~(conts >> (l0 + 1)));  // a run ends with its block: within the 33 slots
+    if (len == BT) whole |= 1ull << l0;
+    else loose |= ((1ull << len) - 1) << l0;
+  }
+  for (int k = 0; k < wave; k++) loose &= loose - 1;
+  while (loose) {  // a row a wavefront
+    const int l = __builtin_ctzll(loose);
+    int64_t vb;
+    int vo;
+    split_slot(slot_of(l), bt, vb, vo);
+    uint16_t *out = v_dst + ((size_t)vb * a.kv_heads + h) * ((size_t)D * bt) + vo;
+#pragma unroll
+    for (int d = lane; d < D; d += 64) {
+      uint16_t x;
+      if (l <= BT) {
+        x = lv[l - 1][d];
+      } else {
+        x = src[(i0 - 1 + l) * a.v_stride + d];
+        if (f16) x = f32_to_f16_bits(bf16_lo(x));
+      }
+      out[(size_t)d * bt] = x;
+    }
+    for (int j = 0; j < 4; j++) loose &= loose - 1;
+  }
+  for (; whole; whole &= whole - 1) {
+    const int l0 = __builtin_ctzll(whole);
+    if (l0 != 1) {
+      load_rows(i0 - 1 + l0);
+      __syncthreads();  // the rows before these have been read
+      rows_to_lds();
+    }
+    uint16_t *out = v_dst + ((size_t)(slot_of(l0) / BT) * a.kv_heads + h) * (D * BT);
+#pragma unroll
+    for (int r = 0; r < D * 2 / 256; r++) {
+      const int d = (r * 256 + tid) >> 1, half = tid & 1;
+      u32x4_t o;
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+        o[x] = (uint32_t)lv[8 * half + 2 * x][d] | ((uint32_t)lv[8 * half + 2 * x + 1][d] << 16);
+      *reinterpret_cast<u32x4_t *>(out + d * BT + 8 * half) = o;
+    }
+  }
+}
+
+// GP: groups of lanes that share a token's rows out.  row_wgs: workgroups of rows.
+template <int D, int PAIRS, int GP>
+__global__ __launch_bounds__(256) void qk_rope_kernel(const QkRopeArgs a, int row_wgs, int aligned) {
+  constexpr int LT = D / 8;
+  constexpr int TOKENS = 256 / LT / GP;  // of a workgroup
+  constexpr int FLIGHT = 3;              // rows of a group in flight
+  if ((int)blockIdx.x >= row_wgs) {
+    const int x = blockIdx.x - row_wgs;
+    values_to_pool<D>(a, x / a.kv_heads, x % a.kv_heads, aligned & 2);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int c = tid % LT, group = tid / LT;
+  const int i = blockIdx.x * TOKENS + group / GP;
+  const bool live = i < a.n;
+  const int token = min(i, a.n - 1);
+  const int R = a.rotary_dim;
+  const bool turned = 8 * c < R;
+  const int heads = a.q_heads + a.kv_heads + (a.v_out ? a.kv_heads : 0);
+  u32x4_t raw[FLIGHT];
+  auto load_rows = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < FLIGHT; k++) {
+      const int h = min(h0 + k * GP, heads - 1);
+      const uint16_t *src = h < a.q_heads ? a.q + token * a.q_stride + (size_t)h * D
+                            : h < a.q_heads + a.kv_heads
+                                ? a.k + token * a.k_stride + (size_t)(h - a.q_heads) * D
+                                : a.v + token * a.v_stride + (size_t)(h - a.q_heads - a.kv_heads) * D;
+      raw[k] = load8_any(src + 8 * c, h < a.q_heads + a.kv_heads || (aligned & 2));
+    }
+  };
+  load_rows(group % GP);  // in flight behind the angles
+  float cs[8], sn[8];
+  if (R > 0) {
+    const int pos = a.positions[token];
+    const int f0 = PAIRS == kAdjacent ? 4 * c : (8 * c) % (R / 2);  // R / 2 is a multiple of 8
+    float freq[8];
+#pragma unroll
+    for (int e = 0; e < (PAIRS == kAdjacent ? 4 : 8); e++) freq[e] = turned ? a.inv_freq[f0 + e] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (PAIRS == kAdjacent && (e & 1)) continue;
+      turn(pos, freq[PAIRS == kAdjacent ? e / 2 : e], cs[e], sn[e]);
+      if (PAIRS == kAdjacent) {
+        cs[e + 1] = cs[e];
+        sn[e + 1] = sn[e];
+        sn[e] = -sn[e];
+      } else if (8 * c < R / 2) {
+        sn[e] = -sn[e];
+      }
+    }
+  }
+  const int partner = 8 * c < R / 2 ? lane + R / 16 : turned ? lane - R / 16 : lane;
+  float wq[8] = {}, wk[8] = {};
+  if (a.q_weight) unpack8(load8(a.q_weight + 8 * c), wq);
+  if (a.k_weight) unpack8(load8(a.k_weight + 8 * c), wk);
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    wq[e] += a.offset;
+    wk[e] += a.offset;
+  }
+  // the key's row of kv head 0 in the pool
+  uint16_t *k_row = nullptr;
+  if (a.slots) {
+    const int64_t slot = a.slots[token];
+    int64_t blk;
+    int off;
+    split_slot(slot, a.pool.block_tokens, blk, off);
+    if (slot >= 0 && blk < a.pool.n_blocks)
+      k_row = static_cast<uint16_t *>(a.k_dst) + ((size_t)blk * a.kv_heads * a.pool.block_tokens + off) * D;
+    else if (live && group % GP == 0 && c == 0)
+      atomicOr(a.err, kErrBadBlock);
+  }
+  for (int h0 = group % GP; h0 < heads; h0 += GP * FLIGHT) {
+    if (h0 >= GP) load_rows(h0);
+#pragma unroll
+    for (int k = 0; k < FLIGHT; k++) {
+      const int h = h0 + k * GP;
+      const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
+      float y[8];
+      unpack8(raw[k], y);
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) sum += y[e] * y[e];
+      sum = row_sum16(sum);
+      if constexpr (LT == 32) sum += xor16_other(sum, lane);
+      if (!is_v && (is_q ? a.q_weight : a.k_weight)) {
+        const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = y[e] * inv * (is_q ? wq[e] : wk[e]);
+      }
+      if (R > 0) {
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          z[e] = PAIRS == kAdjacent ? y[e ^ 1]
+                 : PAIRS == kHalves ? __shfl(y[e], partner)
+                 : LT == 32         ? xor16_other(y[e], lane)
+                                    : dpp<0x128>(y[e]);  // row_ror 8
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = turned && !is_v ? y[e] * cs[e] + z[e] * sn[e] : y[e];
+      }
+      if (!live || h >= heads) continue;
+      u32x4_t w;
+#pragma unroll
+      for (int e = 0; e < 4; e++) w[e] = pack_bf16(y[2 * e], y[2 * e + 1]);
+      if (is_q) {
+        store8_any(a.q_out + ((size_t)i * a.q_heads + h) * D + 8 * c, w, aligned & 1);
+      } else if (is_v) {
+        store8_any(a.v_out + ((size_t)i * a.kv_heads + (h - a.q_heads - a.kv_heads)) * D + 8 * c, raw[k], aligned & 1);
+      } else if (a.k_out) {
+        store8_any(a.k_out + ((size_t)i * a.kv_heads + (h - a.q_heads)) * D + 8 * c, w, aligned & 1);
+      } else if (k_row) {
+        store8_any(k_row + (size_t)(h - a.q_heads) * a.pool.block_tokens * D + 8 * c,
+                   a.pool.format == kF16 ? to_f16(w) : w, true);
+      }
+    }
+  }
+}
+
+template <int D, int PAIRS, int GP>
+void launch_rope_t(const QkRopeArgs &a, int aligned, hipStream_t s) {
+  constexpr int TOKENS = 256 / (D / 8) / GP;
+  const int row_wgs = (a.n + TOKENS - 1) / TOKENS;
+  const int value_wgs = a.k_out ? 0 : (a.n + kFastBlockTokens - 1) / kFastBlockTokens * a.kv_heads;
+  hipLaunchKernelGGL((qk_rope_kernel<D, PAIRS, GP>), dim3(row_wgs + value_wgs), dim3(256), 0, s, a, row_wgs, aligned);
+}
+
+template <int D>
+void launch_rope_d(const QkRopeArgs &a, int aligned, hipStream_t s) {
+  // Few tokens: one a workgroup, its rows side by side.
+  const bool many = a.n >= 512;
+  constexpr int ALL = 256 / (D / 8);
+  if (a.adjacent) {
+    if (many) launch_rope_t<D, kAdjacent, 4>(a, aligned, s);
+    else launch_rope_t<D, kAdjacent, ALL>(a, aligned, s);
+  } else if (a.rotary_dim == D) {
+    if (many) launch_rope_t<D, kFull, 4>(a, aligned, s);
+    else launch_rope_t<D, kFull, ALL>(a, aligned, s);
+  } else {
+    if (many) launch_rope_t<D, kHalves, 4>(a, aligned, s);
+    else launch_rope_t<D, kHalves, ALL>(a, aligned, s);
+  }
+}
+
 }  // namespace
 
 hipError_t launch_qk_rope(const QkRopeArgs &a, hipStream_t s) {
   if (a.n <= 0) return hipSuccess;
+  // Which kernel runs depends on the queries' and keys' rows alone, so that a key's bits do not
+  // depend on where it or the values go.
+  const auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  if ((a.head_dim == 128 || a.head_dim == 256) && a.rotary_dim % 16 == 0 && at16(a.q) && at16(a.k) &&
+      a.q_stride % 8 == 0 && a.k_stride % 8 == 0 && at16(a.q_weight) && at16(a.k_weight)) {
+    const int aligned = (at16(a.q_out) && at16(a.k_out) && at16(a.v_out) ? 1 : 0) |
+                        (at16(a.v) && a.v_stride % 8 == 0 ? 2 : 0);
+    if (a.head_dim == 128) launch_rope_d<128>(a, aligned, s);
+    else launch_rope_d<256>(a, aligned, s);
+    return hipGetLastError();
+  }
   const bool values = a.v_out || !a.k_out;
   hipLaunchKernelGGL(qk_rope_generic_kernel, dim3(a.n, a.q_heads + a.kv_heads * (values ? 2 : 1)), dim3(64), 0, s, a);
   return hipGetLastError();

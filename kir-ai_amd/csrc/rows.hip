@@ -607,6 +607,27 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
   merge_splits<D, false>(a, sq, b, kvh, G, row0, live, 0, kSplitGroup, n_groups);
 }
 
+// Merge of the n <= N splits of one (query row, head): every partial row in flight at
+// once, the (max, sum) pairs one per lane, split weights through v_readlane.
+template <int D, int N>
+__device__ __forceinline__ void rows_merge(const RowsArgs &a, size_t prow, size_t orow, int last, int d) {
+  const size_t p0 = prow * a.max_splits;
+  float o_sp[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) o_sp[i] = a.ws_o[(p0 + min(i, last)) * D + d];
+  const int li = d & 63;
+  const float2 ml = a.ws_ml[p0 + min(li, last)];
+  const float mx[1] = {li <= last ? ml.x : -INFINITY}, ly[1] = {ml.y};
+  float f[1];
+  const float ll = merge_weights<1>(mx, ly, li, f);
+  float oo = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i++)  // nothing of the places past the last (0 x infinity is NaN)
+    oo += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[0]), i)) * (i <= last ? o_sp[i] : 0.0f);
+  const float inv = row_inv(a, ll);
+  a.out[orow * D + d] = f32_to_bf16_rne(gated(oo * inv, a.gate, orow * D + d));
+}
+
 template <int D, int UK>
 __global__ __launch_bounds__(D) void paged_rows_merge_kernel(const RowsArgs a) {
   const int b = blockIdx.y;
@@ -615,7 +636,12 @@ __global__ __launch_bounds__(D) void paged_rows_merge_kernel(const RowsArgs a) {
   if (sq.skip || tok >= sq.chunk || sq.n_splits <= 1) return;
   const size_t prow = (size_t)b * a.max_rows * a.q_heads + blockIdx.x;  // row of the partials
   const size_t orow = (size_t)sq.c0 * a.q_heads + blockIdx.x;           // and of the output
-  rows_merge<D>(a, prow, orow, sq.n_splits - 1, threadIdx.x);
+  const int last = sq.n_splits - 1;
+  const int d = threadIdx.x;
+  if (last < 8) return rows_merge<D, 8>(a, prow, orow, last, d);
+  if (last < 16) return rows_merge<D, 16>(a, prow, orow, last, d);
+  if (last < 32) return rows_merge<D, 32>(a, prow, orow, last, d);
+  return rows_merge<D, kRowsMaxSplits>(a, prow, orow, last, d);
 }
 
 template <int D, int FMT, int PARTS, bool SCORES = false>

@@ -1,5 +1,4 @@
-// The keys of a sequence, their split and the splits' merge in the packed-row kernels (rows.hip,
-// weights.hip).
+// The keys of a sequence and their split in the packed-row kernels (rows.hip, weights.hip).
 #pragma once
 
 #include "wave_ops.h"
@@ -42,35 +41,6 @@ __device__ __forceinline__ SeqSplit seq_split(const RowsArgs &a, int b) {
 // decode kernels in the calls that are theirs too.
 __device__ __forceinline__ float row_inv(const RowsArgs &a, float ll) {
   return ll == 0.0f && (a.chunk_starts || a.zero_bad || a.scores) ? 0.0f : 1.0f / ll;
-}
-
-// Merge of the n <= N splits of one (query row, head): every partial row in flight at
-// once, the (max, sum) pairs one per lane, split weights through v_readlane.
-template <int D, int N>
-__device__ __forceinline__ void rows_merge_n(const RowsArgs &a, size_t prow, size_t orow, int last, int d) {
-  const size_t p0 = prow * a.max_splits;
-  float o_sp[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) o_sp[i] = a.ws_o[(p0 + min(i, last)) * D + d];
-  const int li = d & 63;
-  const float2 ml = a.ws_ml[p0 + min(li, last)];
-  const float mx[1] = {li <= last ? ml.x : -INFINITY}, ly[1] = {ml.y};
-  float f[1];
-  const float ll = merge_weights<1>(mx, ly, li, f);
-  float oo = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; i++)  // nothing of the places past the last (0 x infinity is NaN)
-    oo += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[0]), i)) * (i <= last ? o_sp[i] : 0.0f);
-  const float inv = row_inv(a, ll);
-  a.out[orow * D + d] = f32_to_bf16_rne(gated(oo * inv, a.gate, orow * D + d));
-}
-
-template <int D>
-__device__ __forceinline__ void rows_merge(const RowsArgs &a, size_t prow, size_t orow, int last, int d) {
-  if (last < 8) return rows_merge_n<D, 8>(a, prow, orow, last, d);
-  if (last < 16) return rows_merge_n<D, 16>(a, prow, orow, last, d);
-  if (last < 32) return rows_merge_n<D, 32>(a, prow, orow, last, d);
-  return rows_merge_n<D, kRowsMaxSplits>(a, prow, orow, last, d);
 }
 
 }  // namespace llh

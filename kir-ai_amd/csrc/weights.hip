@@ -16,41 +16,74 @@ namespace llh {
 
 namespace {
 
-constexpr int kWaveKeys = 256;  // positions of a wavefront, four neighbouring ones a lane
 
-// The first `merge_wgs` workgroups of a (kv head, sequence) merge the splits of its rows, the others
-// take kWaveKeys / RW * (wavefronts) positions each: wavefront w takes rows w % RW, w % RW + RW, ...
-// of the positions w / RW, and the RW sums of a position meet in LDS.  Each wavefront finds
-// the (max, sum) of its own rows from the splits' pairs, one a lane; pairs and scores of four rows are
-// in flight together.
-template <int D, int THREADS, int RW>
-__global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsArgs w, int merge_wgs) {
-  constexpr int BATCH = 4;
+// The output of one (query row, head) from the partial rows of its splits, by one wavefront: D / 64
+// dims a lane, eight partials in flight, the pairs one a lane.
+template <int D>
+__device__ __forceinline__ void merge_row(const RowsArgs &a, size_t prow, size_t orow, int n, int lane) {
+  constexpr int PER = D / 64, FLIGHT = 8;
+  typedef __attribute__((ext_vector_type(PER))) float part_t;
+  const float2 ml = a.ws_ml[prow * a.max_splits + min(lane, n - 1)];
+  const part_t *src = reinterpret_cast<const part_t *>(a.ws_o + prow * a.max_splits * D) + lane;
+  part_t o = {};
+  float f[1], sum = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += FLIGHT) {
+    part_t p[FLIGHT];
+#pragma unroll
+    for (int i = 0; i < FLIGHT; i++) p[i] = src[(size_t)min(i0 + i, n - 1) * 64];
+    if (i0 == 0) {
+      const float mx[1] = {lane < n ? ml.x : -INFINITY}, l[1] = {ml.y};
+      sum = merge_weights<1>(mx, l, lane, f);
+    }
+#pragma unroll
+    for (int i = 0; i < FLIGHT; i++)
+      if (i0 + i < n) o += p[i] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[0]), i0 + i));
+  }
+  const float inv = row_inv(a, sum);
+  const size_t at = orow * D + PER * lane;
+#pragma unroll
+  for (int d = 0; d < PER; d++) a.out[at + d] = f32_to_bf16_rne(gated(o[d] * inv, a.gate, at + d));
+}
+
+// The first `tiles` workgroups of a (kv head, sequence) take 64 KPL positions for each wavefront but
+// for those that share them, the others merge the splits of its rows.  Of a tile, wavefront w takes
+// the rows w % RW, w % RW + RW, ... of the positions w / RW, KPL neighbouring ones a lane, BATCH rows in
+// flight, and the RW sums of a position meet in LDS.
+// A row's (max, sum) come from its splits' pairs.  Few rows: each wavefront finds its own rows',
+// a pair a lane.  Many (RW = 16): eight lanes a row, into LDS for the whole workgroup (a wavefront's
+// reduction over 64 lanes for each of its rows took 10 us of 23, up to 256 rows over up to 1732
+// positions, 4 sequences x 2 kv heads).
+template <int D, int THREADS, int RW, int KPL, int BATCH>
+__global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsArgs w, int tiles) {
+  typedef __attribute__((ext_vector_type(KPL))) float keys_t;
+  constexpr int WAVE_KEYS = 64 * KPL;
+  constexpr bool MANY = RW == 16;
+  constexpr int BLOCK = MANY ? 1024 : 1;  // rows whose (max, 1 / sum, position) LDS holds
   const RowsArgs &a = w.rows;
   const int b = blockIdx.z;
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.q_heads / a.pool.kv_heads;
   const SeqSplit sq = seq_split<D == 256 ? 32 : 64>(a, b);
-  if ((int)blockIdx.x < merge_wgs) {
-    constexpr int ROWS = THREADS / D;
-    const int i = blockIdx.x * ROWS + tid / D;
+  if ((int)blockIdx.x >= tiles) {
+    const int i = ((int)blockIdx.x - tiles) * (THREADS / 64) + wave;
     const int tok = i / G;
     if (sq.skip || sq.n_splits <= 1 || tok >= min(sq.chunk, a.max_rows)) return;
     const size_t head = kvh * G + i % G;
-    rows_merge<D>(a, ((size_t)b * a.max_rows + tok) * a.q_heads + head, (size_t)(sq.c0 + tok) * a.q_heads + head,
-                  sq.n_splits - 1, tid % D);
+    merge_row<D>(a, ((size_t)b * a.max_rows + tok) * a.q_heads + head, (size_t)(sq.c0 + tok) * a.q_heads + head,
+                 sq.n_splits, lane);
     return;
   }
   if (sq.flags || (a.chunk_starts && sq.ctx < sq.chunk)) return;  // flagged, or no such call: left alone
-  const int tile0 = ((int)blockIdx.x - merge_wgs) * (THREADS / 64 / RW * kWaveKeys);
+  const int tile0 = (int)blockIdx.x * (THREADS / 64 / RW * WAVE_KEYS);
   if (tile0 >= sq.ctx) return;
-  const int p0 = tile0 + wave / RW * kWaveKeys + 4 * lane;
+  const int wave0 = tile0 + wave / RW * WAVE_KEYS;  // this wavefront's first position
+  const int p0 = wave0 + KPL * lane;
   const size_t at = ((size_t)b * a.pool.kv_heads + kvh) * w.stride + p0;
-  float before[4] = {};
+  float before[KPL] = {};
   if (wave % RW == 0 && w.w_in) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < KPL; i++)
       if (p0 + i < sq.ctx) before[i] = w.w_in[at + i];
   }
   const int rows = max(0, min(sq.chunk, a.max_rows)) * G;
@@ -58,18 +91,76 @@ __global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsAr
   const int base = weights_base(sq.lo);
   const bool here = p0 >= base && p0 < sq.ctx;  // scores of these positions are stored
   const size_t row0 = (size_t)b * a.max_rows * a.q_heads + kvh * G;
-  float acc[4] = {};
-  if (tile0 + wave / RW * kWaveKeys + kWaveKeys > base) {
+  float acc[KPL] = {};
+  // adds row r's weights of this lane's positions, given its scores
+  auto add = [&](const keys_t &s, float m, float inv, int pos) __attribute__((always_inline)) {
+    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+#pragma unroll
+    for (int i = 0; i < KPL; i++) {
+      const int p = p0 + i;
+      acc[i] += (here & (p >= lo) & (p <= pos)) ? fast_exp2(s[i] - m) * inv : 0.0f;
+    }
+  };
+  // the index of row r's scores and pairs
+  auto row_of = [&](int r) __attribute__((always_inline)) { return row0 + (size_t)(r / G) * a.q_heads + r % G; };
+  auto scores_of = [&](size_t row) __attribute__((always_inline)) {
+    return here ? *reinterpret_cast<const keys_t *>(a.scores + row * a.score_stride + (p0 - base)) : keys_t(0.0f);
+  };
+  if constexpr (MANY) {
+    struct Row {
+      float m, inv;
+      int pos, row;  // (row: of the call's rows and heads, which the host keeps below 2^31)
+    };
+    __shared__ Row s_row[BLOCK];
+    if (tile0 + THREADS / 64 / RW * WAVE_KEYS > base) {
+      for (int block = 0; block < rows; block += BLOCK) {
+        const int n = min(BLOCK, rows - block);
+        for (int x = tid / 8; x < n; x += THREADS / 8) {
+          const size_t row = row_of(block + x);
+          const float2 *pairs = a.ws_ml + row * a.max_splits;
+          float2 ml[kRowsMaxSplits / 8];
+          float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kRowsMaxSplits / 8; i++)
+            if (8 * i < sq.n_splits) {
+              ml[i] = pairs[min(8 * i + tid % 8, sq.n_splits - 1)];
+              m = fmaxf(m, ml[i].x);
+            }
+          m = fmaxf(m, dpp<0xB1>(m));
+          m = fmaxf(m, dpp<0x4E>(m));
+          m = fmaxf(m, dpp<0x141>(m));
+          m = m == -INFINITY ? 0.0f : m;  // no key left: every score is -inf
+#pragma unroll
+          for (int i = 0; i < kRowsMaxSplits / 8; i++)
+            if (8 * i < sq.n_splits) sum += 8 * i + tid % 8 < sq.n_splits ? ml[i].y * fast_exp2(ml[i].x - m) : 0.0f;
+          sum = row_sum8(sum);
+          if (tid % 8 == 0)
+            s_row[x] = Row{m, sum == 0.0f ? 0.0f : 1.0f / sum, first + (block + x) / G, (int)(row - row0)};
+        }
+        __syncthreads();
+        for (int r0 = wave % RW; r0 < n; r0 += RW * BATCH) {
+          keys_t s[BATCH];
+#pragma unroll
+          for (int k = 0; k < BATCH; k++) s[k] = scores_of(row0 + s_row[min(r0 + k * RW, n - 1)].row);
+#pragma unroll
+          for (int k = 0; k < BATCH; k++)
+            if (r0 + k * RW < n) {
+              const Row x = s_row[r0 + k * RW];
+              add(s[k], x.m, x.inv, x.pos);
+            }
+        }
+        __syncthreads();
+      }
+    }
+  } else if (wave0 + WAVE_KEYS > base) {
     for (int r0 = wave % RW; r0 < rows; r0 += RW * BATCH) {
       float2 ml[BATCH];
-      float4 s[BATCH];
+      keys_t s[BATCH];
 #pragma unroll
       for (int k = 0; k < BATCH; k++) {
-        const int r = min(r0 + k * RW, rows - 1);
-        const size_t row = row0 + (size_t)(r / G) * a.q_heads + r % G;
+        const size_t row = row_of(min(r0 + k * RW, rows - 1));
         ml[k] = a.ws_ml[row * a.max_splits + min(lane, sq.n_splits - 1)];
-        s[k] = here ? *reinterpret_cast<const float4 *>(a.scores + row * a.score_stride + (p0 - base))
-                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        s[k] = scores_of(row);
       }
 #pragma unroll
       for (int k = 0; k < BATCH; k++) {
@@ -78,32 +169,23 @@ __global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsAr
         const float mx[1] = {lane < sq.n_splits ? ml[k].x : -INFINITY}, l[1] = {ml[k].y};
         float f[1], top;
         const float sum = merge_weights<1>(mx, l, lane, f, &top);
-        const float m = top == -INFINITY ? 0.0f : top;  // no key left: every score is -inf
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int pos = first + r / G;
-        const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int p = p0 + i;
-          acc[i] += (here & (p >= lo) & (p <= pos)) ? fast_exp2((&s[k].x)[i] - m) * inv : 0.0f;
-        }
+        add(s[k], top == -INFINITY ? 0.0f : top, sum == 0.0f ? 0.0f : 1.0f / sum, first + r / G);
       }
     }
   }
   if constexpr (RW > 1) {
-    __shared__ float4 part[THREADS];
-    part[tid] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __shared__ float part[KPL][THREADS];
+#pragma unroll
+    for (int i = 0; i < KPL; i++) part[i][tid] = acc[i];
     __syncthreads();
     if (wave % RW) return;
 #pragma unroll
-    for (int x = 1; x < RW; x++) {
-      const float4 o = part[tid + 64 * x];
+    for (int x = 1; x < RW; x++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[i] += (&o.x)[i];
-    }
+      for (int i = 0; i < KPL; i++) acc[i] += part[i][tid + 64 * x];
   }
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < KPL; i++)
     if (p0 + i < sq.ctx) w.w_out[at + i] = (w.w_in ? w.decay * before[i] : 0.0f) + acc[i];
 }
 
@@ -212,25 +294,29 @@ hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int D, int THREADS, int RW>
+template <int D, int THREADS, int RW, int KPL, int BATCH>
 static hipError_t launch_finish(const WeightsArgs &w, int max_len, hipStream_t s) {
   const RowsArgs &a = w.rows;
-  const int G = a.q_heads / a.pool.kv_heads;
-  const int tile = THREADS / 64 / RW * kWaveKeys;
-  const int merge_wgs = a.max_splits > 1 ? (a.max_rows * G + THREADS / D - 1) / (THREADS / D) : 0;
-  const unsigned tiles = ((unsigned)max_len + tile - 1) / tile;
+  const int rows = a.max_rows * (a.q_heads / a.pool.kv_heads);
+  const int tile = THREADS / 64 / RW * 64 * KPL;
+  const int merge_wgs = a.max_splits > 1 ? (rows + THREADS / 64 - 1) / (THREADS / 64) : 0;
+  const int tiles = (int)(((unsigned)max_len + tile - 1) / tile);
   if (merge_wgs + tiles == 0) return hipSuccess;
-  hipLaunchKernelGGL((weights_finish_kernel<D, THREADS, RW>), dim3(merge_wgs + tiles, a.pool.kv_heads, a.num_seqs),
-                     dim3(THREADS), 0, s, w, merge_wgs);
+  hipLaunchKernelGGL((weights_finish_kernel<D, THREADS, RW, KPL, BATCH>),
+                     dim3(tiles + merge_wgs, a.pool.kv_heads, a.num_seqs), dim3(THREADS), 0, s, w, tiles);
   return hipGetLastError();
 }
 
+// Many rows are shared between wavefronts, and their positions, as one compute unit takes some 50 GB/s,
+// spread over more workgroups.  Measured on MI355X (us, this launch), up to 256 rows of a kv head
+// over up to 1732 positions, 4 x 2 of them: 16 wavefronts sharing 256 positions 11.8, 128 10.0, 64 12.5; 8
+// sharing 256 15.8, 128 13.5.
 template <int D>
 static hipError_t launch_finish_d(const WeightsArgs &w, int max_len, hipStream_t s) {
   const int rows = w.rows.max_rows * (w.rows.q_heads / w.rows.pool.kv_heads);
-  if (rows <= 4) return launch_finish<D, 256, 1>(w, max_len, s);
-  if (rows <= 16) return launch_finish<D, 256, 4>(w, max_len, s);
-  return launch_finish<D, 1024, 16>(w, max_len, s);
+  if (rows <= 4) return launch_finish<D, 256, 1, 4, 4>(w, max_len, s);
+  if (rows <= 16) return launch_finish<D, 256, 4, 4, 4>(w, max_len, s);
+  return launch_finish<D, 1024, 16, 2, 16>(w, max_len, s);
 }
 
 hipError_t launch_weights_finish(const WeightsArgs &w, int max_len, hipStream_t s) {
