@@ -483,7 +483,7 @@ size_t llh_weights_workspace_bytes(int32_t num_seqs, int32_t max_chunk_len, int3
  *   d_kept_lens int32 [num_seqs]: min(len_b, budget) -- the sequence's length after llh_kv_compact;
  *             not d_seq_lens itself
  * A length above max_seq_len is flagged (2), keeps nothing and reports 0.  Calls with a
- * max_seq_len above 32768 keep counts in the stream's workspace (about 1.5 bytes a position). */
+ * max_seq_len above 32768 keep counts in the stream's workspace (about 4.5 bytes a position). */
 typedef struct llh_kv_select_desc {
   int32_t num_seqs;
   int32_t kv_heads;

@@ -54,6 +54,17 @@ __device__ __forceinline__ int wave_inclusive(int v) {
   return v;
 }
 
+// Largest v of the wavefront, the same way.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // Sum of the wavefronts' numbers before this one's.
 template <int WAVES>
 __device__ __forceinline__ int waves_before(const int *s_waves, int wave) {
@@ -240,169 +251,205 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const SelectArgs a) 
   write_kept<THREADS, KPT>(key, r, 0, threshold, want, 0, 0, keep, s_waves);
 }
 
-// Longer rows: tiles of kTileKeys positions, a launch per digit and one that writes.  Every tile
-// leaves its histogram (16-bit counts, two a word) in the workspace, and every workgroup of the
-// next launch adds up the row's: no counter has to be cleared, and nothing depends on order.
+// Longer rows: tiles of kTileKeys positions and three launches.  The first leaves every tile's
+// histogram of the first digit (16-bit counts, two a word) in the workspace; in the second every
+// workgroup adds up its row's, finds the digit and leaves the tile's keys of that digit, a few per cent
+// of them as a rule; in the third every workgroup finds the threshold among the row's such keys and writes
+// its tile's positions.  No counter has to be cleared, and nothing depends on order.  Keys of the
+// digit that are all equal (weights that are all zero, say) are recognised by their least and largest;
+// where they differ and are yet most of a long row, the third launch reads them all in every workgroup
+// (two rows of 1048576 positions: 26 us all equal, 37 spread, 1.3 ms read so).
 constexpr int kTileThreads = 1024;
+constexpr int kTileWaves = kTileThreads / 64;
 constexpr int kTileKpt = 8;
 constexpr int kTileKeys = kTileThreads * kTileKpt;
 constexpr int kTileWords = kBins / 2;
-struct TileState {
-  int digit[2], want[2];  // after the first and the second digit
+struct TileCounts {
+  int larger;  // keys of a larger first digit
+  int cands;   // keys of the digit
+  uint32_t not_least, largest;  // of those: ~ the least, the largest (0 and 0: none)
 };
 struct TileView {
-  uint32_t *hist;    // [rows][tiles][3][kTileWords]
-  int *larger;       // [rows][tiles][2]: keys of the tile larger by the first / second digit
-  TileState *state;  // [rows]
+  uint32_t *hist;      // [rows][tiles][kTileWords]
+  uint32_t *cand;      // [rows][tiles][kTileKeys]
+  TileCounts *counts;  // [rows][tiles]
+  int2 *state;         // [rows] the first digit, and how many of its keys are wanted
 };
 __host__ __device__ inline size_t tile_bytes(size_t rows, size_t tiles) {
-  return rows * tiles * (3 * kTileWords + 2) * 4 + rows * sizeof(TileState);
+  return rows * tiles * ((kTileWords + kTileKeys) * 4 + sizeof(TileCounts)) + rows * sizeof(int2);
 }
 __host__ __device__ inline TileView tile_view(void *ws, size_t rows, size_t tiles) {
   TileView v;
   v.hist = static_cast<uint32_t *>(ws);
-  v.larger = reinterpret_cast<int *>(v.hist + rows * tiles * 3 * kTileWords);
-  v.state = reinterpret_cast<TileState *>(v.larger + rows * tiles * 2);
+  v.cand = v.hist + rows * tiles * kTileWords;
+  v.counts = reinterpret_cast<TileCounts *>(v.cand + rows * tiles * kTileKeys);
+  v.state = reinterpret_cast<int2 *>(v.counts + rows * tiles);
   return v;
 }
 
-// This thread's two bins of the row's histogram of one digit, the larger first.
-__device__ __forceinline__ void row_counts(const uint32_t *hist, int tiles, int (&c)[2]) {
-  c[0] = c[1] = 0;
-  const uint32_t *p = hist + (kTileWords - 1 - threadIdx.x);
-#pragma unroll 8
-  for (int t = 0; t < tiles; t++) {
-    const uint32_t w = p[(size_t)t * 3 * kTileWords];
-    c[0] += (int)(w >> 16);
-    c[1] += (int)(w & 0xffffu);
-  }
-}
+enum { kTileHist, kTileCands, kTileWrite };
 
-// PASS 0, 1, 2: the histogram of that digit; 3: the positions.
-template <int PASS>
+template <int STEP>
 __global__ __launch_bounds__(kTileThreads) void kv_select_tile_kernel(const SelectArgs a) {
   const int tile = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RowRange r = row_range(a, b);
   const size_t row = (size_t)b * a.kv_heads + h;
   int32_t *keep = a.keep + row * a.keep_stride;
-  if (PASS == 3 && tid == 0 && h == 0 && tile == 0) row_lengths(a, b, r.len);
+  if (STEP == kTileWrite && tid == 0 && h == 0 && tile == 0) row_lengths(a, b, r.len);
   const int p0 = tile * kTileKeys;
   if (row_is_plain(a, r.len)) {
-    if (PASS == 3 && r.len <= a.max_seq_len)
+    if (STEP == kTileWrite && r.len <= a.max_seq_len)
       for (int i = p0 + tid; i < min(r.len, p0 + kTileKeys); i += kTileThreads) keep[i] = i;
     return;
   }
-  if (p0 >= r.len) return;
+  if (p0 >= r.len || (STEP != kTileWrite && r.want == 0)) return;
   const int tiles = (r.len + kTileKeys - 1) / kTileKeys;
   const TileView v = tile_view(a.scratch, (size_t)a.num_seqs * a.kv_heads, gridDim.x);
-  uint32_t *const hist_row = v.hist + row * gridDim.x * 3 * kTileWords;
+  const size_t tile_row = row * gridDim.x;
   __shared__ int hist[kBins];
-  __shared__ __attribute__((aligned(16))) int s_waves[kTileThreads / 64];
+  __shared__ __attribute__((aligned(16))) int s_waves[kTileWaves];
   __shared__ int s_found[3];
-  __shared__ int s_before[2][kTileThreads / 64];
+  __shared__ int2 s_before[kTileWaves];
+  __shared__ uint2 s_ends[kTileWaves];
   uint32_t key[kTileKpt];
   load_keys<kTileThreads, kTileKpt>(key, a.weights + row * a.weights_stride, r, p0);
   const int first = p0 + wave * 64 * kTileKpt + lane;
+  auto clear = [&]() __attribute__((always_inline)) {
+    hist[tid] = 0;
+    hist[tid + kTileThreads] = 0;
+    __syncthreads();
+  };
 
-  // the digits so far
-  uint32_t prefix = 0, mask = 0;
-  int want = r.want;
-  if (want > 0) {
-    if (PASS >= 2) {
-      const TileState s = v.state[row];
-      prefix = (uint32_t)s.digit[0] << kDigitShift[0];
-      mask = kDigitMask[0] << kDigitShift[0];
-      want = s.want[0];
-      if (PASS == 3) {
-        prefix |= (uint32_t)s.digit[1] << kDigitShift[1];
-        mask |= kDigitMask[1] << kDigitShift[1];
-        want = s.want[1];
-      }
-    }
-    if (PASS >= 1) {
-      int c[2];
-      row_counts(hist_row + (PASS - 1) * kTileWords, tiles, c);
-      bool all;
-      const int digit = find_digit<kTileThreads, 2>(c, kBins - 1, &want, &all, s_waves, s_found);
-      const uint32_t old_prefix = prefix, old_mask = mask;
-      prefix |= (uint32_t)digit << kDigitShift[PASS - 1];
-      mask |= kDigitMask[PASS - 1] << kDigitShift[PASS - 1];
-      if (PASS < 3) {
-        if (tile == 0 && tid == 0) {
-          v.state[row].digit[PASS - 1] = digit;
-          v.state[row].want[PASS - 1] = want;
-        }
-        // keys that are larger by this digit
-        int n = 0;
+  if constexpr (STEP == kTileHist) {
+    clear();
 #pragma unroll
-        for (int i = 0; i < kTileKpt; i++) {
-          const int p = first + 64 * i;
-          n += __builtin_popcountll(
-              __ballot(p >= r.lo && p < r.hi && (key[i] & old_mask) == old_prefix && (key[i] & mask) > prefix));
-        }
-        if (lane == 0) s_before[0][wave] = n;
-        __syncthreads();
-        if (tid == 0) {
-          int all = 0;
-          for (int w = 0; w < kTileThreads / 64; w++) all += s_before[0][w];
-          v.larger[(row * gridDim.x + tile) * 2 + PASS - 1] = all;
-        }
-      }
+    for (int i = 0; i < kTileKpt; i++) {
+      const int p = first + 64 * i;
+      count_digit(hist, (int)(key[i] >> kDigitShift[0]), p >= r.lo && p < r.hi, lane);
     }
-    if (PASS < 3) {
-      for (int i = tid; i < kBins; i += kTileThreads) hist[i] = 0;
-      __syncthreads();
+    __syncthreads();
+    v.hist[(tile_row + tile) * kTileWords + tid] = (uint32_t)hist[2 * tid] | ((uint32_t)hist[2 * tid + 1] << 16);
+  } else if constexpr (STEP == kTileCands) {
+    int c[2] = {0, 0};
+    const uint32_t *words = v.hist + tile_row * kTileWords + (kTileWords - 1 - tid);
+#pragma unroll 8
+    for (int t = 0; t < tiles; t++) {
+      const uint32_t w = words[(size_t)t * kTileWords];
+      c[0] += (int)(w >> 16);
+      c[1] += (int)(w & 0xffffu);
+    }
+    int want = r.want;
+    bool all;
+    const uint32_t digit = (uint32_t)find_digit<kTileThreads, 2>(c, kBins - 1, &want, &all, s_waves, s_found);
+    if (tile == 0 && tid == 0) v.state[row] = make_int2((int)digit, want);
+    int larger = 0, n = 0;
+    uint32_t mine = 0;
+    uint2 ends = make_uint2(0, 0);
 #pragma unroll
-      for (int i = 0; i < kTileKpt; i++) {
-        const int p = first + 64 * i;
-        count_digit(hist, (int)((key[i] >> kDigitShift[PASS % 3]) & kDigitMask[PASS % 3]),
-                    p >= r.lo && p < r.hi && (key[i] & mask) == prefix, lane);
-      }
-      __syncthreads();
-      hist_row[((size_t)tile * 3 + PASS) * kTileWords + tid] = (uint32_t)hist[2 * tid] | ((uint32_t)hist[2 * tid + 1] << 16);
+    for (int i = 0; i < kTileKpt; i++) {
+      const int p = first + 64 * i;
+      const uint32_t d = key[i] >> kDigitShift[0];
+      const bool mid = p >= r.lo && p < r.hi;
+      larger += __builtin_popcountll(__ballot(mid && d > digit));
+      n += __builtin_popcountll(__ballot(mid && d == digit));
+      mine |= mid && d == digit ? 1u << i : 0u;
+      ends.x = max(ends.x, mid && d == digit ? ~key[i] : 0u);
+      ends.y = max(ends.y, mid && d == digit ? key[i] : 0u);
+    }
+    ends = make_uint2(wave_umax(ends.x), wave_umax(ends.y));
+    if (lane == 0) {
+      s_before[wave] = make_int2(larger, n);
+      s_ends[wave] = ends;
+    }
+    __syncthreads();
+    int at = 0, all_larger = 0, all_n = 0;
+#pragma unroll
+    for (int w = 0; w < kTileWaves; w++) {
+      at += w < wave ? s_before[w].y : 0;
+      all_larger += s_before[w].x;
+      all_n += s_before[w].y;
+      ends.x = max(ends.x, s_ends[w].x);
+      ends.y = max(ends.y, s_ends[w].y);
+    }
+    if (tid == 0) v.counts[tile_row + tile] = TileCounts{all_larger, all_n, ends.x, ends.y};
+    uint32_t *cand = v.cand + (tile_row + tile) * kTileKeys;
+#pragma unroll
+    for (int i = 0; i < kTileKpt; i++) {
+      const bool k = mine >> i & 1;
+      const uint64_t m = __ballot(k);
+      if (k) cand[at + __builtin_popcountll(m & ((1ull << lane) - 1))] = key[i];
+      at += __builtin_popcountll(m);
     }
   } else {
-    prefix = 0xffffffffu;  // nothing of the middle: no key reaches it
-  }
-  if (PASS < 3) return;
-
-  // kept and equal positions of the tiles before this one, a tile per wavefront
-  int larger = 0, equal = 0;
-  if (r.want > 0) {
-    const int digit = (int)(prefix & kDigitMask[2]);
-    for (int t = wave; t < tile; t += kTileThreads / 64) {
-      const uint32_t *ht = hist_row + ((size_t)t * 3 + 2) * kTileWords;
-      if (lane == 0) {
-        const int *l = &v.larger[(row * gridDim.x + t) * 2];
-        larger += l[0] + l[1];
+    uint32_t threshold = 0xffffffffu;  // nothing of the middle: no key reaches it
+    int want = 0, n_larger = 0, n_equal = 0;
+    if (r.want > 0) {
+      const int2 state = v.state[row];
+      uint32_t prefix = (uint32_t)state.x << kDigitShift[0], mask = kDigitMask[0] << kDigitShift[0];
+      want = state.y;
+      // f(key, in the row, tile) for the row's keys of the digit, a tile per wavefront at a time
+      auto for_cands = [&](auto f) __attribute__((always_inline)) {
+        for (int t = wave; t < tiles; t += kTileWaves) {
+          const int n = v.counts[tile_row + t].cands;
+          const uint32_t *cand = v.cand + (tile_row + t) * kTileKeys;
+          for (int i = lane; i < ((n + 63) & ~63); i += 64) f(cand[min(i, n - 1)], i < n, t);
+        }
+      };
+      // the tiles' counts, a tile a lane (every wavefront for itself: no barrier)
+      int larger = 0, equal = 0;  // of the tiles before this one
+      uint2 ends = make_uint2(0, 0);
+      for (int t = lane; t < tiles; t += 64) {
+        const TileCounts c = v.counts[tile_row + t];
+        ends.x = max(ends.x, c.not_least);
+        ends.y = max(ends.y, c.largest);
+        larger += t < tile ? c.larger : 0;
+        equal += t < tile ? c.cands : 0;
       }
-      for (int i = lane; i < 1024 / 2; i += 64) {  // the last digit has ten bits
-        const uint32_t w = ht[i];
-        const int lo_bin = 2 * i, hi_bin = 2 * i + 1;
-        larger += (lo_bin > digit ? (int)(w & 0xffffu) : 0) + (hi_bin > digit ? (int)(w >> 16) : 0);
-        equal += (lo_bin == digit ? (int)(w & 0xffffu) : 0) + (hi_bin == digit ? (int)(w >> 16) : 0);
+      larger = __builtin_amdgcn_readlane(wave_inclusive(larger), 63);
+      equal = __builtin_amdgcn_readlane(wave_inclusive(equal), 63);
+      n_larger = larger;
+      ends = make_uint2(wave_umax(ends.x), wave_umax(ends.y));
+      if (~ends.x == ends.y) {
+        threshold = ends.y;
+        n_equal = equal;
+      } else {
+        bool all = false;
+#pragma unroll
+        for (int pass = 1; pass < 3; pass++) {
+          if (all) break;
+          clear();
+          for_cands([&](uint32_t k, bool on, int) __attribute__((always_inline)) {
+            count_digit(hist, (int)((k >> kDigitShift[pass]) & kDigitMask[pass]), on && (k & mask) == prefix, lane);
+          });
+          __syncthreads();
+          const int c[2] = {hist[kBins - 1 - 2 * tid], hist[kBins - 2 - 2 * tid]};
+          const int digit = find_digit<kTileThreads, 2>(c, kBins - 1, &want, &all, s_waves, s_found);
+          prefix |= (uint32_t)digit << kDigitShift[pass];
+          mask |= kDigitMask[pass] << kDigitShift[pass];
+        }
+        threshold = prefix;
+        if (all) {
+          threshold = prefix - 1;
+          want = 0;
+        }
+        larger = equal = 0;
+        for_cands([&](uint32_t k, bool on, int t) __attribute__((always_inline)) {
+          larger += __builtin_popcountll(__ballot(on && t < tile && k > threshold));
+          equal += __builtin_popcountll(__ballot(on && t < tile && k == threshold));
+        });
+        if (lane == 0) s_before[wave] = make_int2(larger, equal);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kTileWaves; w++) {
+          n_larger += s_before[w].x;
+          n_equal += s_before[w].y;
+        }
       }
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      larger += __shfl_xor(larger, d);
-      equal += __shfl_xor(equal, d);
-    }
+    const int n_out = min(p0, r.lo) + max(0, p0 - r.hi) + n_larger + min(n_equal, want);
+    write_kept<kTileThreads, kTileKpt>(key, r, p0, threshold, want, n_out, n_equal, keep, s_waves);
   }
-  if (lane == 0) {
-    s_before[0][wave] = larger;
-    s_before[1][wave] = equal;
-  }
-  __syncthreads();
-  int n_larger = 0, n_equal = 0;
-#pragma unroll
-  for (int w = 0; w < kTileThreads / 64; w++) {
-    n_larger += s_before[0][w];
-    n_equal += s_before[1][w];
-  }
-  const int n_out = min(p0, r.lo) + max(0, p0 - r.hi) + n_larger + min(n_equal, want);
-  write_kept<kTileThreads, kTileKpt>(key, r, p0, prefix, want, n_out, n_equal, keep, s_waves);
 }
 
 // ---------------------------------------------------------------------------
@@ -713,10 +760,9 @@ hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s) {
     return hipGetLastError();
   }
   const dim3 tiles((n + kTileKeys - 1) / kTileKeys, a.kv_heads, a.num_seqs);
-  hipLaunchKernelGGL(kv_select_tile_kernel<0>, tiles, dim3(kTileThreads), 0, s, a);
-  hipLaunchKernelGGL(kv_select_tile_kernel<1>, tiles, dim3(kTileThreads), 0, s, a);
-  hipLaunchKernelGGL(kv_select_tile_kernel<2>, tiles, dim3(kTileThreads), 0, s, a);
-  hipLaunchKernelGGL(kv_select_tile_kernel<3>, tiles, dim3(kTileThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_select_tile_kernel<kTileHist>, tiles, dim3(kTileThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_select_tile_kernel<kTileCands>, tiles, dim3(kTileThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_select_tile_kernel<kTileWrite>, tiles, dim3(kTileThreads), 0, s, a);
   return hipGetLastError();
 }
 
