@@ -109,6 +109,14 @@ int llh_ctx_reserve_workspace(llh_ctx *ctx, size_t bytes);
  * calls of at most this size allocate nothing (prefill calls that split their keys
  * have scratch of their own: llh_paged_prefill). */
 int llh_ctx_reserve_stream_workspace(llh_ctx *ctx, void *stream, size_t bytes);
+/* Allocates one stream's scratch of the operators around the cache (attention weights, selection in
+ * long rows, norms into quantised pools) now: it is apart from the workspace above, a call that
+ * finds too little gets a further buffer, and none moves or goes before llh_ctx_release_stream, so that
+ * captured graphs stay valid.  A call under capture that finds too little is LLH_ERR_CAPACITY: reserve
+ * (llh_weights_workspace_bytes, llh_kv_select_workspace_bytes, llh_qk_rope_workspace_bytes), or make the
+ * call once, before.  Graphs captured on one stream share its scratch: replay them, and that
+ * stream's calls, one after the other.  hipStreamPerThread has none: LLH_ERR_UNSUPPORTED. */
+int llh_ctx_reserve_ops_workspace(llh_ctx *ctx, void *stream, size_t bytes);
 /* Frees one stream's workspace (after waiting for the device).  Call it before
  * destroying a stream that made batched calls on this context. */
 int llh_ctx_release_stream(llh_ctx *ctx, void *stream);
@@ -437,9 +445,12 @@ int llh_qk_norm_rope(llh_ctx *ctx, const llh_qk_rope_desc *desc, void *d_q_out, 
  * llh_qk_norm_rope followed by llh_kv_append(d_slots, keys, values) (so a key is rounded to bf16
  * before a quantised or fp16 pool's own rounding, and errors are flagged as there; slots of one
  * call are distinct).  bf16 and fp16 pools take one launch; the others keep the rows in the
- * stream's workspace between two.  num_kv_heads and head_dim must be the pool's. */
+ * stream's scratch between two.  num_kv_heads and head_dim must be the pool's. */
 int llh_qk_norm_rope_append(llh_ctx *ctx, llh_kv_pool *pool, const llh_qk_rope_desc *desc, const int64_t *d_slots,
                             void *d_q_out, void *stream);
+
+/* Scratch bytes of that (0 for nothing). */
+size_t llh_qk_rope_workspace_bytes(int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim);
 
 /* ------------------------------------------------------------------ */
 /* attention that says where its weight went, and eviction by it       */
@@ -455,7 +466,7 @@ int llh_qk_norm_rope_append(llh_ctx *ctx, llh_kv_pool *pool, const llh_qk_rope_d
  * every pool format, head_dim <= 512.  A key in a block outside the pool is masked (and flagged),
  * a query that is left with no key gives a zero row and adds nothing, and a non-finite score
  * is flagged.  A sequence that is flagged for its length gets neither output nor weights.
- * The scores pass through the stream's workspace: llh_weights_workspace_bytes. */
+ * The scores pass through the stream's scratch: llh_weights_workspace_bytes. */
 int llh_paged_decode_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_decode_desc *desc, const void *d_q,
                              void *d_out, float score_scale, const float *d_weights_in, float *d_weights_out,
                              int64_t weights_stride, float decay, void *stream);
@@ -469,7 +480,7 @@ int llh_paged_prefill_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_p
                               int32_t max_context_len, const void *d_q, void *d_out, float score_scale,
                               const float *d_weights_in, float *d_weights_out, int64_t weights_stride, float decay,
                               void *stream);
-/* Workspace bytes of either call (max_chunk_len = 1: a decode step), for any split. */
+/* Scratch bytes of either call (max_chunk_len = 1: a decode step), for any split. */
 size_t llh_weights_workspace_bytes(int32_t num_seqs, int32_t max_chunk_len, int32_t num_q_heads, int32_t head_dim,
                                    int32_t max_context_len);
 
@@ -483,7 +494,7 @@ size_t llh_weights_workspace_bytes(int32_t num_seqs, int32_t max_chunk_len, int3
  *   d_kept_lens int32 [num_seqs]: min(len_b, budget) -- the sequence's length after llh_kv_compact;
  *             not d_seq_lens itself
  * A length above max_seq_len is flagged (2), keeps nothing and reports 0.  Calls with a
- * max_seq_len above 32768 keep counts in the stream's workspace (about 4.5 bytes a position). */
+ * max_seq_len above 16384 may keep keys in the stream's scratch (about 4.5 bytes a position). */
 typedef struct llh_kv_select_desc {
   int32_t num_seqs;
   int32_t kv_heads;
@@ -497,6 +508,8 @@ typedef struct llh_kv_select_desc {
 } llh_kv_select_desc;
 int llh_kv_select(llh_ctx *ctx, const llh_kv_select_desc *desc, const float *d_weights, int32_t *d_keep,
                   int32_t *d_kept_lens, void *stream);
+/* Scratch bytes of that (0 where a workgroup holds a row). */
+size_t llh_kv_select_workspace_bytes(int32_t num_seqs, int32_t kv_heads, int32_t max_seq_len);
 
 /* Moves the kept tokens to the front of other blocks: token i of kv head h of sequence b becomes
  * the one at position d_keep[b][h][i] (each head keeps its own), for i < d_kept_lens[b], and with

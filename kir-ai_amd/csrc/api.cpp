@@ -323,12 +323,7 @@ int llh_ctx_destroy(llh_ctx *ctx) {
       (void)hipEventDestroy(ev.second);
     }
   for (hipEvent_t e : ctx->event_pool) (void)hipEventDestroy(e);
-  for (auto &w : ctx->workspaces) {
-    if (w->ptr) (void)hipFree(w->ptr);
-    for (void *p : w->prefill)
-      if (p) (void)hipFree(p);
-    if (w->err) (void)hipFree(w->err);
-  }
+  for (auto &w : ctx->workspaces) w->free_scratch();
   if (ctx->d_err) (void)hipFree(ctx->d_err);
   delete ctx;
   return LLH_OK;
@@ -358,6 +353,17 @@ int llh_ctx_reserve_workspace(llh_ctx *ctx, size_t bytes) {
     if (st != LLH_OK) return st;
   }
   return LLH_OK;
+}
+
+int llh_ctx_reserve_ops_workspace(llh_ctx *ctx, void *stream, size_t bytes) {
+  if (!ctx) return LLH_ERR_NULL;
+  return guarded(ctx, [&]() -> int {
+    const DeviceGuard on(ctx);
+    if (on.status != hipSuccess) return ctx->hip_fail(on.status, "hipSetDevice");
+    WsLease lease;
+    char *base = nullptr;
+    return lease.acquire_ops(ctx, static_cast<hipStream_t>(stream), bytes, &base);
+  });
 }
 
 int llh_ctx_reserve_stream_workspace(llh_ctx *ctx, void *stream, size_t bytes) {
@@ -393,13 +399,10 @@ static int release_slot(llh_ctx *ctx, hipStream_t stream, bool stream_alive) {
     std::lock_guard<std::mutex> g2(ctx->ws_mu);
     ctx->retired_flags |= flags;
   }
-  if (w->ptr) (void)hipFree(w->ptr);
-  for (void *&p : w->prefill) {
-    if (p) (void)hipFree(p);
-    p = nullptr;
-  }
-  if (w->err) (void)hipFree(w->err);
+  w->free_scratch();
   w->ptr = nullptr;
+  for (void *&p : w->prefill) p = nullptr;
+  w->ops.clear();
   w->err = nullptr;
   w->bytes = w->prefill_bytes = 0;
   return LLH_OK;
@@ -468,7 +471,7 @@ int llh_ctx_metrics(const llh_ctx *ctx, llh_metrics *out) {
   std::lock_guard<std::mutex> g(const_cast<llh_ctx *>(ctx)->ws_mu);
   out->stream_slots = ctx->workspaces.size();
   out->workspace_bytes = 0;
-  for (auto &w : ctx->workspaces) out->workspace_bytes += w->bytes + w->prefill_bytes;
+  for (auto &w : ctx->workspaces) out->workspace_bytes += w->bytes + w->prefill_bytes + w->ops_bytes();
   return LLH_OK;
 }
 
@@ -1395,8 +1398,11 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   const size_t sc_off = ml_off + align_up(rows * sr.max_splits * sizeof(float2));
   const int64_t sc_stride = score_stride(span);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const DeviceGuard on(ctx);
+  if (on.status != hipSuccess) return ctx->hip_fail(on.status, "hipSetDevice");
   WsLease lease;
-  const int st = lease.acquire(ctx, s, sc_off + rows * sc_stride * sizeof(float));
+  char *ws = nullptr;
+  const int st = lease.acquire_ops(ctx, s, sc_off + rows * sc_stride * sizeof(float), &ws);
   if (st != LLH_OK) return st;
   WeightsArgs w{};
   RowsArgs &r = w.rows;
@@ -1406,8 +1412,8 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   r.chunk_starts = c.chunk_starts;
   r.context_lens = c.lens;
   r.tables = c.tables;
-  r.ws_o = reinterpret_cast<float *>(lease.base());
-  r.ws_ml = reinterpret_cast<float2 *>(lease.base() + ml_off);
+  r.ws_o = reinterpret_cast<float *>(ws);
+  r.ws_ml = reinterpret_cast<float2 *>(ws + ml_off);
   r.err = lease.err();
   r.num_seqs = c.num_seqs;
   r.max_rows = c.max_rows;
@@ -1423,7 +1429,7 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   r.scale = score_scale;
   r.scale_log2e = score_scale * 1.4426950408889634f;
   r.gate = static_cast<const uint16_t *>(c.gate);
-  r.scores = reinterpret_cast<float *>(lease.base() + sc_off);
+  r.scores = reinterpret_cast<float *>(ws + sc_off);
   r.score_stride = (int32_t)sc_stride;
   w.w_in = d_in;
   w.w_out = d_w;
@@ -1456,15 +1462,17 @@ int llh_paged_decode_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_de
                              void *d_out, float score_scale, const float *d_weights_in, float *d_weights_out,
                              int64_t weights_stride, float decay, void *stream) {
   if (!ctx || !pool || !desc) return LLH_ERR_NULL;
-  int st = check_desc_common(ctx, pool, desc->num_seqs, desc->num_q_heads, desc->max_blocks_per_seq, desc->window);
-  if (st != LLH_OK || desc->num_seqs == 0) return st;
-  if (desc->max_seq_len < 0) return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_seq_len must be >= 0");
-  st = check_span(ctx, pool, desc->max_seq_len, desc->window, desc->max_blocks_per_seq);
-  if (st != LLH_OK) return st;
-  const WeightsCall c{desc->num_seqs, 1, desc->num_q_heads, desc->max_blocks_per_seq, desc->window, desc->max_seq_len,
-                      desc->total_tokens_hint, nullptr, desc->d_seq_lens, desc->d_block_tables, desc->d_gate};
-  return weights_impl(ctx, pool, c, d_q, d_out, score_scale, d_weights_in, d_weights_out, weights_stride, decay,
-                      stream);
+  return guarded(ctx, [&]() -> int {
+    int st = check_desc_common(ctx, pool, desc->num_seqs, desc->num_q_heads, desc->max_blocks_per_seq, desc->window);
+    if (st != LLH_OK || desc->num_seqs == 0) return st;
+    if (desc->max_seq_len < 0) return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_seq_len must be >= 0");
+    st = check_span(ctx, pool, desc->max_seq_len, desc->window, desc->max_blocks_per_seq);
+    if (st != LLH_OK) return st;
+    const WeightsCall c{desc->num_seqs, 1, desc->num_q_heads, desc->max_blocks_per_seq, desc->window, desc->max_seq_len,
+                        desc->total_tokens_hint, nullptr, desc->d_seq_lens, desc->d_block_tables, desc->d_gate};
+    return weights_impl(ctx, pool, c, d_q, d_out, score_scale, d_weights_in, d_weights_out, weights_stride, decay,
+                        stream);
+  });
 }
 
 int llh_paged_prefill_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_prefill_desc *desc,
@@ -1472,21 +1480,23 @@ int llh_paged_prefill_weights(llh_ctx *ctx, const llh_kv_pool *pool, const llh_p
                               const float *d_weights_in, float *d_weights_out, int64_t weights_stride, float decay,
                               void *stream) {
   if (!ctx || !pool || !desc) return LLH_ERR_NULL;
-  int st = check_desc_common(ctx, pool, desc->num_seqs, desc->num_q_heads, desc->max_blocks_per_seq, desc->window);
-  if (st != LLH_OK || desc->num_seqs == 0) return st;
-  if (desc->total_q_rows < 0 || desc->max_chunk_len <= 0 || max_context_len < 0)
-    return ctx->fail(LLH_ERR_INVALID_SHAPE, "row counts must be >= 0 and chunks at least one row");
-  if (desc->max_chunk_len > LLH_WEIGHTS_MAX_CHUNK) {
-    ctx->not_handled++;
-    return ctx->fail(LLH_ERR_UNSUPPORTED,
-                     "attention weights take at most " + std::to_string(LLH_WEIGHTS_MAX_CHUNK) + " rows a sequence");
-  }
-  if (!desc->d_chunk_starts) return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
-  const WeightsCall c{desc->num_seqs, desc->max_chunk_len, desc->num_q_heads, desc->max_blocks_per_seq, desc->window,
-                      max_context_len, 0, desc->d_chunk_starts, desc->d_context_lens, desc->d_block_tables,
-                      desc->d_gate};
-  return weights_impl(ctx, pool, c, d_q, d_out, score_scale, d_weights_in, d_weights_out, weights_stride, decay,
-                      stream);
+  return guarded(ctx, [&]() -> int {
+    int st = check_desc_common(ctx, pool, desc->num_seqs, desc->num_q_heads, desc->max_blocks_per_seq, desc->window);
+    if (st != LLH_OK || desc->num_seqs == 0) return st;
+    if (desc->total_q_rows < 0 || desc->max_chunk_len <= 0 || max_context_len < 0)
+      return ctx->fail(LLH_ERR_INVALID_SHAPE, "row counts must be >= 0 and chunks at least one row");
+    if (desc->max_chunk_len > LLH_WEIGHTS_MAX_CHUNK) {
+      ctx->not_handled++;
+      return ctx->fail(LLH_ERR_UNSUPPORTED,
+                       "attention weights take at most " + std::to_string(LLH_WEIGHTS_MAX_CHUNK) + " rows a sequence");
+    }
+    if (!desc->d_chunk_starts) return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
+    const WeightsCall c{desc->num_seqs, desc->max_chunk_len, desc->num_q_heads, desc->max_blocks_per_seq, desc->window,
+                        max_context_len, 0, desc->d_chunk_starts, desc->d_context_lens, desc->d_block_tables,
+                        desc->d_gate};
+    return weights_impl(ctx, pool, c, d_q, d_out, score_scale, d_weights_in, d_weights_out, weights_stride, decay,
+                        stream);
+  });
 }
 
 int llh_debug_gather(llh_ctx *ctx, const llh_kv_pool *pool, const llh_decode_desc *desc, int32_t seq, int32_t lo,

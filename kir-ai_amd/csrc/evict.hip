@@ -742,8 +742,16 @@ void launch_compact_d(const CompactArgs &a, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
+// Whether rows are selected from in tiles: beyond what a workgroup's registers hold, and somewhat below
+// where there are few rows.  Measured on MI355X, a workgroup a row / tiles (us): 8 rows of 16384 18.2 /
+// 24.6, 24000 28.7 / 25.3, 32768 33.3 / 24.7; 64 rows of 32768 33.7 / 27.8; 256 rows 37.7 / 99.7.
+static bool select_in_tiles(int num_seqs, int kv_heads, int max_seq_len) {
+  return max_seq_len > 1024 * kSelectMaxKpt ||
+         (max_seq_len > 1024 * kSelectMaxKpt / 2 && (long long)num_seqs * kv_heads <= 64);
+}
+
 size_t select_scratch_bytes(int num_seqs, int kv_heads, int max_seq_len) {
-  if (max_seq_len <= 1024 * kSelectMaxKpt) return 0;
+  if (!select_in_tiles(num_seqs, kv_heads, max_seq_len)) return 0;
   return tile_bytes((size_t)num_seqs * kv_heads, (max_seq_len + kTileKeys - 1) / kTileKeys);
 }
 
@@ -751,7 +759,7 @@ hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s) {
   if (a.num_seqs <= 0) return hipSuccess;
   const int n = a.max_seq_len;
   const dim3 grid(a.kv_heads, a.num_seqs);
-  if (n <= 1024 * kSelectMaxKpt) {
+  if (!select_in_tiles(a.num_seqs, a.kv_heads, n)) {
     if (n <= 1024) hipLaunchKernelGGL((kv_select_kernel<256, 4>), grid, dim3(256), 0, s, a);
     else if (n <= 4096) hipLaunchKernelGGL((kv_select_kernel<1024, 4>), grid, dim3(1024), 0, s, a);
     else if (n <= 8192) hipLaunchKernelGGL((kv_select_kernel<1024, 8>), grid, dim3(1024), 0, s, a);

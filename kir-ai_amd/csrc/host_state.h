@@ -57,6 +57,22 @@ struct StreamWorkspace {
   // and never moved or freed before the slot is.
   void *prefill[kPrefillScratches] = {};
   size_t prefill_bytes = 0;
+  // Scratch of the operators around the cache (attention weights, selection, norms into quantised
+  // pools), apart from `ptr` and never moved: a call that needs more gets a further, larger buffer,
+  // and the ones before it stay until the slot goes, so what a captured graph holds stays valid.
+  std::vector<std::pair<void *, size_t>> ops;  // the last is the largest
+  size_t ops_bytes() const {
+    size_t n = 0;
+    for (auto &b : ops) n += b.second;
+    return n;
+  }
+  void free_scratch() {
+    if (ptr) (void)hipFree(ptr);
+    for (void *p : prefill)
+      if (p) (void)hipFree(p);
+    for (auto &b : ops) (void)hipFree(b.first);
+    if (err) (void)hipFree(err);
+  }
   // arrival counters of the launches that merge their own partials, in err's allocation: zero between
   // launches (the launches of a stream run one after the other; each leaves them zero).
   // None to a call under capture, whose graph may be replayed on another stream beside this
@@ -213,6 +229,26 @@ struct llh_ctx {
   }
 };
 
+// The context's device as the current one for the length of a call: a launch on the null stream
+// goes to the current device.
+struct DeviceGuard {
+  int before = -1;
+  hipError_t status;
+  explicit DeviceGuard(const llh_ctx *ctx) {
+    int now = -1;
+    status = hipGetDevice(&now);
+    if (status == hipSuccess && now != ctx->device) {
+      status = hipSetDevice(ctx->device);
+      if (status == hipSuccess) before = now;
+    }
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+  DeviceGuard(const DeviceGuard &) = delete;
+  DeviceGuard &operator=(const DeviceGuard &) = delete;
+};
+
 // A batched call's hold on its stream's workspace: locks the slot for the
 // lifetime of the lease (through the call's last launch).
 struct WsLease {
@@ -248,12 +284,67 @@ struct WsLease {
     w->prefill_bytes += bytes;
     return static_cast<char *>(p);
   }
+  // `bytes` of the slot's `ops` scratch at *base.  Nothing is allocated under capture: the call before it
+  // (or llh_ctx_reserve_ops_workspace) has to.
+  int acquire_ops(llh_ctx *ctx, hipStream_t s, size_t bytes, char **base) {
+    if (s == hipStreamPerThread)
+      return ctx->fail(LLH_ERR_UNSUPPORTED, "hipStreamPerThread is another stream in every thread: this call keeps "
+                                            "scratch by stream and takes one of its own");
+    const bool capturing = llh::StreamWorkspace::capturing(s);
+    if (capturing) {
+      std::lock_guard<std::mutex> g(ctx->ws_mu);
+      for (auto &x : ctx->workspaces)
+        if (x->stream == s) w = x;
+    } else {
+      w = ctx->slot(s);
+      if (!w) return ctx->fail(LLH_ERR_DEVICE, "stream error word allocation failed");
+    }
+    if (w) lock = std::unique_lock<std::mutex>(w->mu);
+    if (w && !w->ops.empty() && w->ops.back().second >= bytes) {
+      *base = static_cast<char *>(w->ops.back().first);
+      return LLH_OK;
+    }
+    if (capturing)
+      return ctx->fail(LLH_ERR_CAPACITY, "the stream's scratch must be reserved before capture "
+                                         "(llh_ctx_reserve_ops_workspace)");
+    // at least twice the last: the buffers together stay below twice the largest
+    size_t nb = bytes;
+    if (!w->ops.empty()) nb = std::max(nb, 2 * w->ops.back().second);
+    nb = llh::align_up(std::max(nb, llh::kAlign));
+    w->ops.reserve(w->ops.size() + 1);
+    void *p = nullptr;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e == hipSuccess) e = hipMalloc(&p, nb);
+    if (e != hipSuccess && nb > llh::align_up(bytes)) {  // not twice the last, then
+      (void)hipGetLastError();
+      nb = llh::align_up(std::max(bytes, llh::kAlign));
+      e = hipMalloc(&p, nb);
+    }
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return ctx->hip_fail(e, "hipMalloc(workspace)");
+    }
+    w->ops.emplace_back(p, nb);
+    *base = static_cast<char *>(p);
+    return LLH_OK;
+  }
   int32_t *err() const { return w->err; }
   int32_t *counters() const { return w->counters(); }
   char *base() const { return static_cast<char *>(w->ptr); }
 };
 
 namespace llh {
+
+// Runs a C entry point's body: no exception leaves it.
+template <typename F>
+int guarded(llh_ctx *ctx, F body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    ctx->device_errors++;
+    return LLH_ERR_DEVICE;
+  }
+}
 
 // A decode step planned on the host: the kernel choice and the byte layout of
 // its workspace (offsets from the workspace base, `bytes` in all).  Shared by

@@ -358,6 +358,7 @@ SIGNATURES = {
     "llh_ctx_last_error": (ctypes.c_char_p, [_P]),
     "llh_ctx_reserve_workspace": (ctypes.c_int, [_P, _SZ]),
     "llh_ctx_reserve_stream_workspace": (ctypes.c_int, [_P, _P, _SZ]),
+    "llh_ctx_reserve_ops_workspace": (ctypes.c_int, [_P, _P, _SZ]),
     "llh_ctx_release_stream": (ctypes.c_int, [_P, _P]),
     "llh_ctx_set_option": (ctypes.c_int, [_P, _I32, _I32]),
     "llh_ctx_get_option": (ctypes.c_int, [_P, _I32, ctypes.POINTER(_I32)]),
@@ -387,6 +388,8 @@ SIGNATURES = {
                                                 ctypes.c_int64, ctypes.c_float, _P]),
     "llh_paged_prefill_weights": (ctypes.c_int, [_P, _P, ctypes.POINTER(PrefillDesc), _I32, _P, _P, ctypes.c_float, _P,
                                                  _P, ctypes.c_int64, ctypes.c_float, _P]),
+    "llh_qk_rope_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
+    "llh_kv_select_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
     "llh_weights_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
     "llh_kv_select": (ctypes.c_int, [_P, ctypes.POINTER(KvSelectDesc), _P, _P, _P, _P]),
     "llh_kv_compact": (ctypes.c_int, [_P, _P, ctypes.POINTER(KvCompactDesc), _P]),
@@ -590,6 +593,18 @@ class Context:
     def reserve_stream_workspace(self, nbytes: int, stream=None) -> None:
         self.check(self.lib.llh_ctx_reserve_stream_workspace(self.handle, _stream(stream), nbytes))
 
+    def reserve_ops_workspace(self, nbytes: int, stream=None) -> None:
+        """Scratch of attention weights, long selections and norms into quantised pools, ahead of time."""
+        self.check(self.lib.llh_ctx_reserve_ops_workspace(self.handle, self._own_stream(stream), nbytes))
+
+    def _own_stream(self, stream):
+        """The given stream, or this context's device's current one."""
+        if stream is None:
+            import torch
+
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return _stream(stream)
+
     def release_stream(self, stream) -> None:
         self.check(self.lib.llh_ctx_release_stream(self.handle, _stream(stream)))
 
@@ -773,12 +788,12 @@ class Context:
     def qk_norm_rope(self, desc: QkRopeDesc, q_out, k_out, stream=None) -> None:
         """llh_qk_norm_rope: per-head norms and rotation of queries and keys."""
         self.check(self.lib.llh_qk_norm_rope(self.handle, ctypes.byref(desc), _ptr(q_out), _ptr(k_out),
-                                             _stream(stream)))
+                                             self._own_stream(stream)))
 
     def qk_norm_rope_append(self, pool: "KvPool", desc: QkRopeDesc, slots, q_out, stream=None) -> None:
         """llh_qk_norm_rope_append: the same, with keys and values written to the pool's slots (int64 [tokens])."""
         self.check(self.lib.llh_qk_norm_rope_append(self.handle, pool.handle, ctypes.byref(desc), _ptr(slots),
-                                                    _ptr(q_out), _stream(stream)))
+                                                    _ptr(q_out), self._own_stream(stream)))
 
     def paged_decode_weights(self, pool: "KvPool", desc: DecodeDesc, q, out, score_scale: float, weights_in,
                              weights_out, decay: float = 1.0, stream=None) -> None:
@@ -787,7 +802,7 @@ class Context:
         self._check_weights(weights_in, weights_out)
         self.check(self.lib.llh_paged_decode_weights(
             self.handle, pool.handle, ctypes.byref(desc), _ptr(q), _ptr(out), score_scale, _ptr(weights_in),
-            _ptr(weights_out), weights_out.shape[-1], decay, _stream(stream)))
+            _ptr(weights_out), weights_out.shape[-1], decay, self._own_stream(stream)))
 
     def paged_prefill_weights(self, pool: "KvPool", desc: PrefillDesc, max_context_len: int, q, out,
                               score_scale: float, weights_in, weights_out, decay: float = 1.0, stream=None) -> None:
@@ -795,7 +810,7 @@ class Context:
         self._check_weights(weights_in, weights_out)
         self.check(self.lib.llh_paged_prefill_weights(
             self.handle, pool.handle, ctypes.byref(desc), max_context_len, _ptr(q), _ptr(out), score_scale,
-            _ptr(weights_in), _ptr(weights_out), weights_out.shape[-1], decay, _stream(stream)))
+            _ptr(weights_in), _ptr(weights_out), weights_out.shape[-1], decay, self._own_stream(stream)))
 
     @staticmethod
     def _check_weights(weights_in, weights_out) -> None:
@@ -804,6 +819,12 @@ class Context:
         for w in (weights_in, weights_out):
             if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or w.shape != weights_out.shape):
                 raise LlhError(ERR_INVALID_SHAPE, "weights are contiguous f32 of one shape")
+
+    def select_workspace_bytes(self, num_seqs: int, kv_heads: int, max_seq_len: int) -> int:
+        return self.lib.llh_kv_select_workspace_bytes(num_seqs, kv_heads, max_seq_len)
+
+    def qk_rope_workspace_bytes(self, num_tokens: int, num_kv_heads: int, head_dim: int) -> int:
+        return self.lib.llh_qk_rope_workspace_bytes(num_tokens, num_kv_heads, head_dim)
 
     def weights_workspace_bytes(self, num_seqs: int, max_chunk_len: int, num_q_heads: int, head_dim: int,
                                 max_context_len: int) -> int:
@@ -822,7 +843,7 @@ class Context:
     def kv_select(self, desc: KvSelectDesc, weights, keep, kept_lens, stream=None) -> None:
         """llh_kv_select: the positions each (sequence, kv head) keeps, ascending, and the lengths that leaves."""
         self.check(self.lib.llh_kv_select(self.handle, ctypes.byref(desc), _ptr(weights), _ptr(keep),
-                                          _ptr(kept_lens), _stream(stream)))
+                                          _ptr(kept_lens), self._own_stream(stream)))
 
     @staticmethod
     def compact_desc(seq_lens, kept_lens, keep, src_tables, dst_tables, max_kept: int, weights_in=None,
@@ -850,7 +871,7 @@ class Context:
 
     def kv_compact(self, pool: "KvPool", desc: KvCompactDesc, stream=None) -> None:
         """llh_kv_compact: the kept tokens (and their weights) to the destination tables' blocks."""
-        self.check(self.lib.llh_kv_compact(self.handle, pool.handle, ctypes.byref(desc), _stream(stream)))
+        self.check(self.lib.llh_kv_compact(self.handle, pool.handle, ctypes.byref(desc), self._own_stream(stream)))
 
     def write_blocks(self, pool: "KvPool", blocks, k, v, stream=None) -> None:
         self.check(
