@@ -1404,8 +1404,7 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   char *ws = nullptr;
   const int st = lease.acquire_ops(ctx, s, sc_off + rows * sc_stride * sizeof(float), &ws);
   if (st != LLH_OK) return st;
-  WeightsArgs w{};
-  RowsArgs &r = w.rows;
+  RowsArgs r{};
   r.pool = pv;
   r.q = static_cast<const uint16_t *>(d_q);
   r.out = static_cast<uint16_t *>(d_out);
@@ -1431,15 +1430,20 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
   r.gate = static_cast<const uint16_t *>(c.gate);
   r.scores = reinterpret_cast<float *>(ws + sc_off);
   r.score_stride = (int32_t)sc_stride;
-  w.w_in = d_in;
-  w.w_out = d_w;
-  w.stride = stride;
-  w.decay = decay;
+  r.w_in = d_in;
+  r.w_out = d_w;
+  r.w_stride = stride;
+  r.decay = decay;
+  // Where no sequence is split and a kv head's rows are one tile, the workgroup that made the scores adds
+  // the weights up: no second launch.  (By the last workgroup of a split sequence it does not pay.)
+  // Measured on MI355X, two launches / one (us), Hq16 / Hkv8, head_dim 128, bf16: 1 x 64 9.4 / 6.6, 1 x 130 11.0 /
+  // 8.1, 16 x 130 11.4 / 8.4; in two and more splits 1 x 300 11.8 / 12.0, 1 x 1000 12.0 / 13.7, 16 x 1000 19.4 / 21.1.
+  r.weights_here = tuned && !c.chunk_starts && r.max_splits == 1 && c.q_heads / pv.kv_heads <= 16;
   (c.chunk_starts ? ctx->prefill_calls : ctx->decode_calls)++;
   if (tuned) ctx->routes[c.chunk_starts ? LLH_ROUTE_ROWS_PREFILL : LLH_ROUTE_ROWS_DECODE]++;
   else (c.chunk_starts ? ctx->generic_prefill_calls : ctx->generic_decode_calls)++;
   hipError_t e = tuned ? launch_rows(r, false, s) : launch_weights_generic(r, s);
-  if (e == hipSuccess) e = launch_weights_finish(w, c.max_ctx, s);
+  if (e == hipSuccess && !r.weights_here) e = launch_weights_finish(r, c.max_ctx, s);
   if (e != hipSuccess) return ctx->hip_fail(e, "attention weights launch");
   return LLH_OK;
 }

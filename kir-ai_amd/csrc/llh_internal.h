@@ -182,19 +182,15 @@ struct RowsArgs {
   // of sequences in one split too
   float *scores;
   int32_t score_stride;     // a multiple of 64
+  const float *w_in;        // [num_seqs][Hkv][w_stride], or null (zeros)
+  float *w_out;
+  int64_t w_stride;
+  float decay;
+  int32_t weights_here;     // 1: the attention launch accumulates (decode, one split, one row tile)
 };
 int rows_unit_keys(int head_dim);
 // Scores are stored from a multiple of 64 positions on, so that units and vectors of keys are whole.
 __host__ __device__ constexpr int weights_base(int lo) { return lo & ~63; }
-
-// Accumulation of the softmax weights over the rows of `rows` (its scores and ws_ml).
-struct WeightsArgs {
-  RowsArgs rows;
-  const float *w_in;        // [num_seqs][Hkv][stride], or null (zeros)
-  float *w_out;
-  int64_t stride;
-  float decay;
-};
 
 // Norms and rotation of queries and keys (qkrope.hip).
 struct QkRopeArgs {
@@ -348,7 +344,7 @@ constexpr int kWeightsMaxDim = 512;
 constexpr int kWeightsMaxLen = 1 << 30;
 hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s);
 // merges the splits and accumulates
-hipError_t launch_weights_finish(const WeightsArgs &a, int max_len, hipStream_t s);
+hipError_t launch_weights_finish(const RowsArgs &a, int max_len, hipStream_t s);
 hipError_t launch_qk_rope(const QkRopeArgs &a, hipStream_t s);
 hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s);
 hipError_t launch_kv_compact(const CompactArgs &a, hipStream_t s);

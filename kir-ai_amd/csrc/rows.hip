@@ -159,7 +159,36 @@ __device__ __forceinline__ void merge_splits(const RowsArgs &a, const SeqSplit &
   }
 }
 
-// SCORES: every score and each row's (max, sum) are stored for weights.hip.
+// The weights of a decode step whose sequences are not split and whose group is one tile, by the
+// workgroup that made the scores; row_ml: the rows' (max, sum) in LDS.  The sums are those of
+// weights_finish_kernel, bit for bit: row after row up to four rows, else four sums of every fourth.
+__device__ __forceinline__ void accumulate_weights(const RowsArgs &a, const SeqSplit &sq, int b, int kvh, int live,
+                                                   const float2 *row_ml) {
+  const size_t row0 = (size_t)b * a.q_heads + kvh * (a.q_heads / a.pool.kv_heads);
+  const size_t w0 = ((size_t)b * a.pool.kv_heads + kvh) * a.w_stride;
+  const float *scores = a.scores + row0 * a.score_stride - weights_base(sq.lo);
+  for (int p = threadIdx.x; p < sq.ctx; p += 64 * WAVES) {
+    const float before = a.w_in ? a.w_in[w0 + p] : 0.0f;
+    float acc[4] = {};
+    if (p >= sq.lo)
+      for (int r0 = 0; r0 < live; r0 += 4) {
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[k] = scores[(size_t)min(r0 + k, live - 1) * a.score_stride + p];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (r0 + k < live) {
+            const float2 ml = row_ml[r0 + k];
+            const float w = score_weight(s[k], ml.x == -INFINITY ? 0.0f : ml.x, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
+            acc[live <= 4 ? 0 : k] += w;
+          }
+      }
+    a.w_out[w0 + p] = accumulated(a, before, live <= 4 ? acc[0] : ((acc[0] + acc[1]) + acc[2]) + acc[3]);
+  }
+}
+
+// SCORES: every score and each row's (max, sum) are stored for weights.hip, or (a.weights_here) for
+// accumulate_weights.
 template <int D, int FMT, int PARTS, bool SCORES = false>
 __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void paged_rows_kernel(const RowsArgs a) {
   static_assert(!SCORES || PARTS > 1 || !is16(FMT), "the sum is that of the weights before any rounding");
@@ -548,6 +577,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
   for (int d = 0; d < ND; d++) *reinterpret_cast<f32x4_t *>(&s_o[wave][col][16 * d + 4 * g]) = oacc[d];
   __syncthreads();
   const int live = min(TILE, rows - row0);
+  __shared__ float2 s_row_ml[SCORES ? TILE : 1];
   for (int i = tid; i < live * (D / 4); i += 64 * WAVES) {
     const int r = i / (D / 4);
     const int d = 4 * (i % (D / 4));
@@ -568,7 +598,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
     if (sq.n_splits == 1) {
       const float inv = row_inv(a, ll);
       if constexpr (SCORES) {
-        if (d == 0)
+        if (d == 0 && a.weights_here) s_row_ml[r] = make_float2(mm, ll);
+        else if (d == 0)
           a.ws_ml[(((size_t)b * a.max_rows + tok) * a.q_heads + head) * a.max_splits] = make_float2(mm, ll);
       }
       const size_t o = ((size_t)(sq.c0 + tok) * a.q_heads + head) * D + d;
@@ -586,6 +617,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 && is16(FMT) ? 1 : 2) void pag
         if (d == 0) a.ws_ml[p] = make_float2(mm, ll);
       }
     }
+  }
+  if constexpr (SCORES) {
+    if (!a.weights_here) return;
+    __syncthreads();  // the scores have been written, and s_row_ml
+    accumulate_weights(a, sq, b, kvh, live, s_row_ml);
+    return;
   }
   if (sq.n_splits <= 1 || !a.counters) return;
   // The last workgroup of the tile merges the splits.  One compute unit takes about 32 GB/s past

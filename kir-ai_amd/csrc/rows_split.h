@@ -43,4 +43,13 @@ __device__ __forceinline__ float row_inv(const RowsArgs &a, float ll) {
   return ll == 0.0f && (a.chunk_starts || a.zero_bad || a.scores) ? 0.0f : 1.0f / ll;
 }
 
+// The weight of a score, given its row's maximum and 1 / sum, and an accumulator's new value: the same
+// bits wherever they are computed.
+__device__ __forceinline__ float score_weight(float s, float m, float inv) {
+  return rounded_product(fast_exp2(s - m), inv);
+}
+__device__ __forceinline__ float accumulated(const RowsArgs &a, float before, float sum) {
+  return a.w_in ? __builtin_fmaf(a.decay, before, sum) : sum;
+}
+
 }  // namespace llh

@@ -54,12 +54,11 @@ __device__ __forceinline__ void merge_row(const RowsArgs &a, size_t prow, size_t
 // reduction over 64 lanes for each of its rows took 10 us of 23, up to 256 rows over up to 1732
 // positions, 4 sequences x 2 kv heads).
 template <int D, int THREADS, int RW, int KPL, int BATCH>
-__global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsArgs w, int tiles) {
+__global__ __launch_bounds__(THREADS) void weights_finish_kernel(const RowsArgs a, int tiles) {
   typedef __attribute__((ext_vector_type(KPL))) float keys_t;
   constexpr int WAVE_KEYS = 64 * KPL;
   constexpr bool MANY = RW == 16;
   constexpr int BLOCK = MANY ? 1024 : 1;  // rows whose (max, 1 / sum, position) LDS holds
-  const RowsArgs &a = w.rows;
   const int b = blockIdx.z;
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -79,12 +78,12 @@ __global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsAr
   if (tile0 >= sq.ctx) return;
   const int wave0 = tile0 + wave / RW * WAVE_KEYS;  // this wavefront's first position
   const int p0 = wave0 + KPL * lane;
-  const size_t at = ((size_t)b * a.pool.kv_heads + kvh) * w.stride + p0;
+  const size_t at = ((size_t)b * a.pool.kv_heads + kvh) * a.w_stride + p0;
   float before[KPL] = {};
-  if (wave % RW == 0 && w.w_in) {
+  if (wave % RW == 0 && a.w_in) {
 #pragma unroll
     for (int i = 0; i < KPL; i++)
-      if (p0 + i < sq.ctx) before[i] = w.w_in[at + i];
+      if (p0 + i < sq.ctx) before[i] = a.w_in[at + i];
   }
   const int rows = max(0, min(sq.chunk, a.max_rows)) * G;
   const int first = sq.ctx - sq.chunk;
@@ -98,7 +97,7 @@ __global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsAr
 #pragma unroll
     for (int i = 0; i < KPL; i++) {
       const int p = p0 + i;
-      acc[i] += (here & (p >= lo) & (p <= pos)) ? fast_exp2(s[i] - m) * inv : 0.0f;
+      acc[i] += (here & (p >= lo) & (p <= pos)) ? score_weight(s[i], m, inv) : 0.0f;
     }
   };
   // the index of row r's scores and pairs
@@ -186,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void weights_finish_kernel(const WeightsAr
   }
 #pragma unroll
   for (int i = 0; i < KPL; i++)
-    if (p0 + i < sq.ctx) w.w_out[at + i] = (w.w_in ? w.decay * before[i] : 0.0f) + acc[i];
+    if (p0 + i < sq.ctx) a.w_out[at + i] = accumulated(a, before[i], acc[i]);
 }
 
 // Attention of one (query row, head) per workgroup for the shapes outside the packed-row kernel:
@@ -295,15 +294,14 @@ hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s) {
 }
 
 template <int D, int THREADS, int RW, int KPL, int BATCH>
-static hipError_t launch_finish(const WeightsArgs &w, int max_len, hipStream_t s) {
-  const RowsArgs &a = w.rows;
+static hipError_t launch_finish(const RowsArgs &a, int max_len, hipStream_t s) {
   const int rows = a.max_rows * (a.q_heads / a.pool.kv_heads);
   const int tile = THREADS / 64 / RW * 64 * KPL;
   const int merge_wgs = a.max_splits > 1 ? (rows + THREADS / 64 - 1) / (THREADS / 64) : 0;
   const int tiles = (int)(((unsigned)max_len + tile - 1) / tile);
   if (merge_wgs + tiles == 0) return hipSuccess;
   hipLaunchKernelGGL((weights_finish_kernel<D, THREADS, RW, KPL, BATCH>),
-                     dim3(tiles + merge_wgs, a.pool.kv_heads, a.num_seqs), dim3(THREADS), 0, s, w, tiles);
+                     dim3(tiles + merge_wgs, a.pool.kv_heads, a.num_seqs), dim3(THREADS), 0, s, a, tiles);
   return hipGetLastError();
 }
 
@@ -312,16 +310,16 @@ static hipError_t launch_finish(const WeightsArgs &w, int max_len, hipStream_t s
 // over up to 1732 positions, 4 x 2 of them: 16 wavefronts sharing 256 positions 11.8, 128 10.0, 64 12.5; 8
 // sharing 256 15.8, 128 13.5.
 template <int D>
-static hipError_t launch_finish_d(const WeightsArgs &w, int max_len, hipStream_t s) {
-  const int rows = w.rows.max_rows * (w.rows.q_heads / w.rows.pool.kv_heads);
-  if (rows <= 4) return launch_finish<D, 256, 1, 4, 4>(w, max_len, s);
-  if (rows <= 16) return launch_finish<D, 256, 4, 4, 4>(w, max_len, s);
-  return launch_finish<D, 1024, 16, 2, 16>(w, max_len, s);
+static hipError_t launch_finish_d(const RowsArgs &a, int max_len, hipStream_t s) {
+  const int rows = a.max_rows * (a.q_heads / a.pool.kv_heads);
+  if (rows <= 4) return launch_finish<D, 256, 1, 4, 4>(a, max_len, s);
+  if (rows <= 16) return launch_finish<D, 256, 4, 4, 4>(a, max_len, s);
+  return launch_finish<D, 1024, 16, 2, 16>(a, max_len, s);
 }
 
-hipError_t launch_weights_finish(const WeightsArgs &w, int max_len, hipStream_t s) {
+hipError_t launch_weights_finish(const RowsArgs &a, int max_len, hipStream_t s) {
   // (other head_dims come in one split: nothing is merged)
-  return w.rows.pool.head_dim == 256 ? launch_finish_d<256>(w, max_len, s) : launch_finish_d<128>(w, max_len, s);
+  return a.pool.head_dim == 256 ? launch_finish_d<256>(a, max_len, s) : launch_finish_d<128>(a, max_len, s);
 }
 
 }  // namespace llh
