@@ -1388,8 +1388,15 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
     const long long total =
         c.total_hint > 0 ? tiles * ((long long)c.total_hint / uk + c.num_seqs) : tiles * units * c.num_seqs;
     sr = split_rows(ctx, pv, tiles * c.num_seqs, units, total, rows, SIZE_MAX);
-  }
-  else {
+    // (one launch, see below, as long as it lasts: a unit more on a workgroup costs about 0.8 us of its
+    // memory rate.  Whole / split (us), Hq16 / Hkv8, bf16: 5 units 10.1 / 11.6, 7 11.1 / 11.5, 10 14.1 / 11.7;
+    // Hq32 / Hkv4 12.0 / 12.5, 13.4 / 12.4; Hq16 / Hkv2, head_dim 256 11.3 / 12.4, 13.4 / 12.7)
+    constexpr int kWholeUnits = 5;
+    if (!c.chunk_starts && group <= 16 && units <= kWholeUnits) {
+      sr.single_units = std::max(sr.single_units, kWholeUnits);
+      sr.max_splits = 1;
+    }
+  } else {
     sr.max_splits = 1;
     sr.single_units = INT32_MAX / 2;
   }
