@@ -444,8 +444,8 @@ int llh_qk_norm_rope(llh_ctx *ctx, const llh_qk_rope_desc *desc, void *d_q_out, 
 /* The same, with the keys and the values written to the cache: the pool's bytes are those of
  * llh_qk_norm_rope followed by llh_kv_append(d_slots, keys, values) (so a key is rounded to bf16
  * before a quantised or fp16 pool's own rounding, and errors are flagged as there; slots of one
- * call are distinct).  bf16 and fp16 pools take one launch; the others keep the rows in the
- * stream's scratch between two.  num_kv_heads and head_dim must be the pool's. */
+ * call are distinct).  bf16 and fp16 pools of 16-token blocks take one launch; others may keep
+ * the rows in the stream's scratch between two.  num_kv_heads and head_dim must be the pool's. */
 int llh_qk_norm_rope_append(llh_ctx *ctx, llh_kv_pool *pool, const llh_qk_rope_desc *desc, const int64_t *d_slots,
                             void *d_q_out, void *stream);
 

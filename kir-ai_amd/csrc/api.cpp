@@ -1358,7 +1358,8 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
                  float score_scale, const float *d_in, float *d_w, int64_t stride, float decay, void *stream) {
   if (!d_q || !d_out || !d_w || !c.lens || !c.tables)
     return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
-  if (c.num_seqs > 65535) return ctx->fail(LLH_ERR_INVALID_SHAPE, "num_seqs must be <= 65535");
+  if (c.num_seqs > 65535 || pool->view.kv_heads > 65535)
+    return ctx->fail(LLH_ERR_INVALID_SHAPE, "num_seqs and kv_heads must be <= 65535");
   if (c.max_ctx > kWeightsMaxLen) return ctx->fail(LLH_ERR_INVALID_SHAPE, "context too long for one call");
   if (stride < std::max(1, c.max_ctx))
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "weights_stride must hold the longest context");

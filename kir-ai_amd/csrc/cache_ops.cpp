@@ -86,6 +86,8 @@ int llh_qk_norm_rope(llh_ctx *ctx, const llh_qk_rope_desc *desc, void *d_q_out, 
     if (on.status != hipSuccess) return ctx->hip_fail(on.status, "hipSetDevice");
     QkRopeArgs a = rope_args(desc, d_q_out);
     a.k_out = static_cast<uint16_t *>(d_k_out);
+    a.v = nullptr;
+    a.v_stride = 0;
     const hipError_t e = launch_qk_rope(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return ctx->hip_fail(e, "norm and rotation launch");
     return LLH_OK;
@@ -110,7 +112,7 @@ int llh_qk_norm_rope_append(llh_ctx *ctx, llh_kv_pool *pool, const llh_qk_rope_d
     const DeviceGuard on(ctx);
     if (on.status != hipSuccess) return ctx->hip_fail(on.status, "hipSetDevice");
     QkRopeArgs a = rope_args(desc, d_q_out);
-    if (is16(pool->view.format)) {
+    if (is16(pool->view.format) && (pool->view.block_tokens == kFastBlockTokens || !qk_rope_pieces(a))) {
       a.slots = d_slots;
       a.pool = pool->view;
       a.k_dst = pool->k;
@@ -121,7 +123,7 @@ int llh_qk_norm_rope_append(llh_ctx *ctx, llh_kv_pool *pool, const llh_qk_rope_d
       if (e != hipSuccess) return ctx->hip_fail(e, "norm, rotation and append launch");
       return LLH_OK;
     }
-    // quantised pools: the bf16 rows in the stream's workspace, then the append kernel
+    // other pools: the bf16 rows in the stream's scratch, then the append kernel
     const size_t bytes = llh_qk_rope_workspace_bytes(desc->num_tokens, desc->num_kv_heads, desc->head_dim) / 2;
     WsLease lease;
     char *ws = nullptr;

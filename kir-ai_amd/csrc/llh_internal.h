@@ -345,6 +345,10 @@ constexpr int kWeightsMaxLen = 1 << 30;
 hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s);
 // merges the splits and accumulates
 hipError_t launch_weights_finish(const RowsArgs &a, int max_len, hipStream_t s);
+// Whether the queries' and keys' rows are taken in 16-byte pieces.  It depends on nothing else, so that a
+// key's bits do not depend on where it or the values go; such rows go straight into 16-token
+// blocks only.
+bool qk_rope_pieces(const QkRopeArgs &a);
 hipError_t launch_qk_rope(const QkRopeArgs &a, hipStream_t s);
 hipError_t launch_kv_select(const SelectArgs &a, hipStream_t s);
 hipError_t launch_kv_compact(const CompactArgs &a, hipStream_t s);

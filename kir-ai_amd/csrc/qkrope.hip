@@ -109,16 +109,19 @@ __device__ __forceinline__ void unpack8(const u32x4_t &w, float (&x)[8]) {
   }
 }
 __device__ __forceinline__ u32x4_t load8(const uint16_t *p) { return *reinterpret_cast<const u32x4_t *>(p); }
-// (outputs and values may lie anywhere: what a row's numbers are does not depend on it)
-__device__ __forceinline__ u32x4_t load8_any(const uint16_t *p, bool aligned) {
-  if (aligned) return load8(p);
+// Outputs and values may lie anywhere (ALIGNED: at 16 bytes): what a row's numbers are does not
+// depend on it.
+template <bool ALIGNED>
+__device__ __forceinline__ u32x4_t load8_any(const uint16_t *p) {
+  if constexpr (ALIGNED) return load8(p);
   u32x4_t w;
 #pragma unroll
   for (int i = 0; i < 4; i++) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
   return w;
 }
-__device__ __forceinline__ void store8_any(uint16_t *p, const u32x4_t &w, bool aligned) {
-  if (aligned) {
+template <bool ALIGNED>
+__device__ __forceinline__ void store8_any(uint16_t *p, const u32x4_t &w) {
+  if constexpr (ALIGNED) {
     *reinterpret_cast<u32x4_t *>(p) = w;
     return;
   }
@@ -135,30 +138,18 @@ __device__ __forceinline__ u32x4_t to_f16(const u32x4_t &w) {
   return r;
 }
 
-// Block and offset of a slot (a division of 64-bit numbers takes a hundred instructions).
-__device__ __forceinline__ void split_slot(int64_t slot, int bt, int64_t &blk, int &off) {
-  if (bt == kFastBlockTokens) {
-    blk = slot >> 4;
-    off = (int)slot & 15;
-  } else {
-    blk = slot / bt;
-    off = (int)(slot % bt);
-  }
-}
-
 // Puts the values of one kv head of 16 tokens into a bf16 or fp16 pool.  V lies dim-major, 16 tokens
 // of a dim side by side, so tokens that fill a whole block are turned in LDS and written 16 bytes a
 // lane; rows of the call that fill a block need not start at a multiple of 16 of them, so a workgroup
 // takes the runs that start in its 16 rows (a run: neighbouring rows in neighbouring slots of one
 // block), wherever they end.  Runs that do not fill a block are written element by element, a
 // row per wavefront.  The 16 rows are loaded beside their slots, which only say where they go.
-template <int D>
-__device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, int h, bool aligned) {
+template <int D, bool ALIGNED>
+__device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, int h) {
   constexpr int BT = kFastBlockTokens;
   constexpr int LT = D / 8, ROUND = 256 / LT;  // lanes a row, rows a round
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i0 = tile * BT;
-  const int bt = a.pool.block_tokens;
   const bool f16 = a.pool.format == kF16;
   uint16_t *const v_dst = static_cast<uint16_t *>(a.v_dst);
   const uint16_t *const src = a.v + (size_t)h * D;
@@ -168,7 +159,7 @@ __device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, in
   auto load_rows = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < BT / ROUND; r++)
-      w[r] = load8_any(src + min(i + r * ROUND + tid / LT, a.n - 1) * a.v_stride + 8 * (tid % LT), aligned);
+      w[r] = load8_any<ALIGNED>(src + min(i + r * ROUND + tid / LT, a.n - 1) * a.v_stride + 8 * (tid % LT));
   };
   auto rows_to_lds = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -180,14 +171,10 @@ __device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, in
   // lane l: the slot of row i0 - 1 + l
   const int i = i0 - 1 + lane;
   const int64_t slot = lane <= 32 && i >= 0 && i < a.n ? a.slots[i] : -1;
-  int64_t blk;
-  int off;
-  split_slot(slot, bt, blk, off);
-  const bool valid = slot >= 0 && blk < a.pool.n_blocks;
+  const bool valid = slot >= 0 && slot / BT < a.pool.n_blocks;
   const int64_t prev = __shfl_up(slot, 1);
   const bool prev_valid = __shfl_up((int)valid, 1) != 0;
-  // (other block sizes have no runs)
-  const bool start = bt != BT || !(lane > 0 && prev_valid && slot == prev + 1) || off == 0;
+  const bool start = !(lane > 0 && prev_valid && slot == prev + 1) || slot % BT == 0;
   if (tid >= 1 && tid <= BT && i < a.n && !valid && h == 0) atomicOr(a.err, kErrBadBlock);
   const uint64_t starts = __ballot(valid && start && lane >= 1 && lane <= BT);
   const uint64_t conts = __ballot(valid && !start);
@@ -208,10 +195,8 @@ __device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, in
   for (int k = 0; k < wave; k++) loose &= loose - 1;
   while (loose) {  // a row a wavefront
     const int l = __builtin_ctzll(loose);
-    int64_t vb;
-    int vo;
-    split_slot(slot_of(l), bt, vb, vo);
-    uint16_t *out = v_dst + ((size_t)vb * a.kv_heads + h) * ((size_t)D * bt) + vo;
+    const int64_t at = slot_of(l);
+    uint16_t *out = v_dst + ((size_t)(at / BT) * a.kv_heads + h) * (D * BT) + at % BT;
 #pragma unroll
     for (int d = lane; d < D; d += 64) {
       uint16_t x;
@@ -221,7 +206,7 @@ __device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, in
         x = src[(i0 - 1 + l) * a.v_stride + d];
         if (f16) x = f32_to_f16_bits(bf16_lo(x));
       }
-      out[(size_t)d * bt] = x;
+      out[d * BT] = x;
     }
     for (int j = 0; j < 4; j++) loose &= loose - 1;
   }
@@ -246,14 +231,15 @@ __device__ __forceinline__ void values_to_pool(const QkRopeArgs &a, int tile, in
 }
 
 // GP: groups of lanes that share a token's rows out.  row_wgs: workgroups of rows.
-template <int D, int PAIRS, int GP>
-__global__ __launch_bounds__(256) void qk_rope_kernel(const QkRopeArgs a, int row_wgs, int aligned) {
+template <int D, int PAIRS, int GP, bool ALIGNED>
+__global__ __launch_bounds__(256) void qk_rope_kernel(const QkRopeArgs a, int row_wgs) {
+  constexpr int BT = kFastBlockTokens;
   constexpr int LT = D / 8;
   constexpr int TOKENS = 256 / LT / GP;  // of a workgroup
   constexpr int FLIGHT = 3;              // rows of a group in flight
   if ((int)blockIdx.x >= row_wgs) {
     const int x = blockIdx.x - row_wgs;
-    values_to_pool<D>(a, x / a.kv_heads, x % a.kv_heads, aligned & 2);
+    values_to_pool<D, ALIGNED>(a, x / a.kv_heads, x % a.kv_heads);
     return;
   }
   const int tid = threadIdx.x, lane = tid & 63;
@@ -273,14 +259,14 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(const QkRopeArgs a, int ro
                             : h < a.q_heads + a.kv_heads
                                 ? a.k + token * a.k_stride + (size_t)(h - a.q_heads) * D
                                 : a.v + token * a.v_stride + (size_t)(h - a.q_heads - a.kv_heads) * D;
-      raw[k] = load8_any(src + 8 * c, h < a.q_heads + a.kv_heads || (aligned & 2));
+      raw[k] = load8_any<ALIGNED>(src + 8 * c);
     }
   };
   load_rows(group % GP);  // in flight behind the angles
   float cs[8], sn[8];
   if (R > 0) {
     const int pos = a.positions[token];
-    const int f0 = PAIRS == kAdjacent ? 4 * c : (8 * c) % (R / 2);  // R / 2 is a multiple of 8
+    const int f0 = PAIRS == kAdjacent ? 4 * c : 8 * c < R / 2 ? 8 * c : 8 * c - R / 2;  // (R / 2: a multiple of 8)
     float freq[8];
 #pragma unroll
     for (int e = 0; e < (PAIRS == kAdjacent ? 4 : 8); e++) freq[e] = turned ? a.inv_freq[f0 + e] : 0.0f;
@@ -310,11 +296,8 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(const QkRopeArgs a, int ro
   uint16_t *k_row = nullptr;
   if (a.slots) {
     const int64_t slot = a.slots[token];
-    int64_t blk;
-    int off;
-    split_slot(slot, a.pool.block_tokens, blk, off);
-    if (slot >= 0 && blk < a.pool.n_blocks)
-      k_row = static_cast<uint16_t *>(a.k_dst) + ((size_t)blk * a.kv_heads * a.pool.block_tokens + off) * D;
+    if (slot >= 0 && slot / BT < a.pool.n_blocks)
+      k_row = static_cast<uint16_t *>(a.k_dst) + ((size_t)(slot / BT) * a.kv_heads * BT + slot % BT) * D;
     else if (live && group % GP == 0 && c == 0)
       atomicOr(a.err, kErrBadBlock);
   }
@@ -352,55 +335,56 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(const QkRopeArgs a, int ro
 #pragma unroll
       for (int e = 0; e < 4; e++) w[e] = pack_bf16(y[2 * e], y[2 * e + 1]);
       if (is_q) {
-        store8_any(a.q_out + ((size_t)i * a.q_heads + h) * D + 8 * c, w, aligned & 1);
+        store8_any<ALIGNED>(a.q_out + ((size_t)i * a.q_heads + h) * D + 8 * c, w);
       } else if (is_v) {
-        store8_any(a.v_out + ((size_t)i * a.kv_heads + (h - a.q_heads - a.kv_heads)) * D + 8 * c, raw[k], aligned & 1);
+        store8_any<ALIGNED>(a.v_out + ((size_t)i * a.kv_heads + (h - a.q_heads - a.kv_heads)) * D + 8 * c, raw[k]);
       } else if (a.k_out) {
-        store8_any(a.k_out + ((size_t)i * a.kv_heads + (h - a.q_heads)) * D + 8 * c, w, aligned & 1);
+        store8_any<ALIGNED>(a.k_out + ((size_t)i * a.kv_heads + (h - a.q_heads)) * D + 8 * c, w);
       } else if (k_row) {
-        store8_any(k_row + (size_t)(h - a.q_heads) * a.pool.block_tokens * D + 8 * c,
-                   a.pool.format == kF16 ? to_f16(w) : w, true);
+        store8_any<true>(k_row + (h - a.q_heads) * (BT * D) + 8 * c, a.pool.format == kF16 ? to_f16(w) : w);
       }
     }
   }
 }
 
-template <int D, int PAIRS, int GP>
-void launch_rope_t(const QkRopeArgs &a, int aligned, hipStream_t s) {
+template <int D, int PAIRS, int GP, bool ALIGNED>
+void launch_rope_t(const QkRopeArgs &a, hipStream_t s) {
   constexpr int TOKENS = 256 / (D / 8) / GP;
   const int row_wgs = (a.n + TOKENS - 1) / TOKENS;
   const int value_wgs = a.k_out ? 0 : (a.n + kFastBlockTokens - 1) / kFastBlockTokens * a.kv_heads;
-  hipLaunchKernelGGL((qk_rope_kernel<D, PAIRS, GP>), dim3(row_wgs + value_wgs), dim3(256), 0, s, a, row_wgs, aligned);
+  hipLaunchKernelGGL((qk_rope_kernel<D, PAIRS, GP, ALIGNED>), dim3(row_wgs + value_wgs), dim3(256), 0, s, a, row_wgs);
+}
+
+// Few tokens: one a workgroup, its rows side by side.
+template <int D, int PAIRS>
+void launch_rope_p(const QkRopeArgs &a, bool aligned, hipStream_t s) {
+  constexpr int ALL = 256 / (D / 8);
+  if (!aligned) launch_rope_t<D, PAIRS, ALL, false>(a, s);
+  else if (a.n >= 512) launch_rope_t<D, PAIRS, 4, true>(a, s);
+  else launch_rope_t<D, PAIRS, ALL, true>(a, s);
 }
 
 template <int D>
-void launch_rope_d(const QkRopeArgs &a, int aligned, hipStream_t s) {
-  // Few tokens: one a workgroup, its rows side by side.
-  const bool many = a.n >= 512;
-  constexpr int ALL = 256 / (D / 8);
-  if (a.adjacent) {
-    if (many) launch_rope_t<D, kAdjacent, 4>(a, aligned, s);
-    else launch_rope_t<D, kAdjacent, ALL>(a, aligned, s);
-  } else if (a.rotary_dim == D) {
-    if (many) launch_rope_t<D, kFull, 4>(a, aligned, s);
-    else launch_rope_t<D, kFull, ALL>(a, aligned, s);
-  } else {
-    if (many) launch_rope_t<D, kHalves, 4>(a, aligned, s);
-    else launch_rope_t<D, kHalves, ALL>(a, aligned, s);
-  }
+void launch_rope_d(const QkRopeArgs &a, bool aligned, hipStream_t s) {
+  if (a.adjacent) launch_rope_p<D, kAdjacent>(a, aligned, s);
+  else if (a.rotary_dim == D) launch_rope_p<D, kFull>(a, aligned, s);
+  else launch_rope_p<D, kHalves>(a, aligned, s);
 }
+
+bool at16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
+bool qk_rope_pieces(const QkRopeArgs &a) {
+  return (a.head_dim == 128 || a.head_dim == 256) && a.rotary_dim % 16 == 0 && at16(a.q) && at16(a.k) &&
+         a.q_stride % 8 == 0 && a.k_stride % 8 == 0 && at16(a.q_weight) && at16(a.k_weight);
+}
+
 hipError_t launch_qk_rope(const QkRopeArgs &a, hipStream_t s) {
   if (a.n <= 0) return hipSuccess;
-  // Which kernel runs depends on the queries' and keys' rows alone, so that a key's bits do not
-  // depend on where it or the values go.
-  const auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-  if ((a.head_dim == 128 || a.head_dim == 256) && a.rotary_dim % 16 == 0 && at16(a.q) && at16(a.k) &&
-      a.q_stride % 8 == 0 && a.k_stride % 8 == 0 && at16(a.q_weight) && at16(a.k_weight)) {
-    const int aligned = (at16(a.q_out) && at16(a.k_out) && at16(a.v_out) ? 1 : 0) |
-                        (at16(a.v) && a.v_stride % 8 == 0 ? 2 : 0);
+  if (qk_rope_pieces(a)) {
+    const bool aligned = at16(a.q_out) && at16(a.k_out) && at16(a.v_out) && at16(a.v) && a.v_stride % 8 == 0;
+    if (!a.k_out && a.pool.block_tokens != kFastBlockTokens) return hipErrorInvalidValue;
     if (a.head_dim == 128) launch_rope_d<128>(a, aligned, s);
     else launch_rope_d<256>(a, aligned, s);
     return hipGetLastError();

@@ -180,6 +180,33 @@ def test_norm_rope_append_is_the_two_calls(ctx, fmt, Hq, Hkv, D, bt, pad):
         assert np.array_equal(a[key], b[key]), key
 
 
+@pytest.mark.parametrize("D", [128, 256])
+def test_norm_rope_append_unaligned_values_and_output(ctx, D):
+    """Values and queries that lie anywhere, keys in 16-byte pieces: the same bits."""
+    import torch
+
+    Hq, Hkv, n = 4, 2, 37
+    qkv, wq, wk, pos, freq = rope_case(n, Hq, Hkv, D, 64, 8)
+    t = view_bf16(qkv)
+    q, k, v = split(t, Hq, Hkv, D)
+    odd = torch.zeros(v.numel() + 1, dtype=torch.bfloat16, device="cuda")
+    odd[1:] = v.reshape(-1)
+    dev = [view_bf16(wq), view_bf16(wk), to_dev(pos), to_dev(freq), to_dev(np.arange(5, 5 + n, dtype=np.int64))]
+    pools = [fresh_pool(ctx, llm_hip.KV_F16, 16, Hkv, D, 3, 90) for _ in range(2)]
+    outs = []
+    for pool, values, off in ((pools[0], v, 0), (pools[1], odd[1:].view(n, Hkv, D), 1)):
+        buf = torch.zeros(n * Hq * D + 1, dtype=torch.bfloat16, device="cuda")
+        d = ctx.qk_rope_desc(q, k, values, dev[2], dev[3], q_weight=dev[0], k_weight=dev[1])
+        ctx.qk_norm_rope_append(pool, d, dev[4], buf[off:])
+        outs.append(buf[off:off + n * Hq * D].clone())
+    torch.cuda.synchronize()
+    assert ctx.device_errors() == 0
+    assert torch.equal(outs[0].view(torch.int16), outs[1].view(torch.int16))
+    a, b = (p.raw() for p in pools)
+    for key in a:
+        assert np.array_equal(a[key], b[key]), key
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "f16", "int8"])
 def test_norm_rope_append_bad_slots(ctx, fmt):
     """Slots outside the pool are flagged and write nothing; the others are written."""
@@ -339,6 +366,27 @@ def test_decode_weights_splits(ctx, fmt, Hq, Hkv, D):
     check_weights(ctx, fmt, [4097], Hq, Hkv, D, window=2049)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 128), (16, 2, 256), (4, 2, 64)])
+@pytest.mark.parametrize("chunk", [False, True])
+def test_weights_over_a_ring_of_blocks(ctx, Hq, Hkv, D, chunk):
+    """A window served by a ring of blocks: positions far past the table row, read modulo its length."""
+    import torch
+
+    window, ring, n = 100, 9, 1003
+    rows = 4 if chunk else 1
+    pool = fresh_pool(ctx, llm_hip.KV_BF16, BT, Hkv, D, 12, 71)
+    table = np.random.default_rng(5).permutation(12)[:ring].astype(np.int32)[None]
+    batch = workloads.PagedBatch(np.array([n], np.int32), table, 12, BT, np.zeros(1, np.int32))
+    q = bf16(73, rows, Hq, D)
+    k, v, live = ref.cached(pool, llm_hip.KV_BF16, BT, Hkv, D, 12, np.resize(table[0], -(-n // BT)), n)
+    want, acc = ref.attend(f(q).astype(np.float64), k, v, live, 1.0 / math.sqrt(D), window)
+    w = torch.full((1, Hkv, n + 1), 0.5, device="cuda")
+    out = run_weights(ctx, pool, batch, table, q, [rows] if chunk else None, window, w, w)
+    assert ctx.device_errors() == 0
+    assert_out(out, want, "ring")
+    assert_weights(w[0, :, :n].cpu().numpy(), 0.5 + acc, "ring")
+
+
 @pytest.mark.parametrize("fmt,Hq,Hkv,D,bt", [("int8_row", 4, 2, 128, 16), ("bf16", 4, 2, 64, 16), ("f16", 4, 4, 96, 8),
                                              ("int8", 6, 2, 80, 16), ("fp8", 4, 1, 64, 32), ("bf16", 2, 1, 512, 16),
                                              ("bf16", 3, 1, 7, 5)])
@@ -490,6 +538,12 @@ def test_select_long(ctx, n, budget):
     """Long rows beside short ones, an odd stride (rows that do not start at 16 bytes)."""
     w = heavy(n, 2, 2, n + 3)
     check_select(ctx, w, [n, n // 3], budget, 4, min(16, budget - 4))
+
+
+def test_select_long_rows_of_many(ctx):
+    """More rows than are cut into tiles, of lengths about what one workgroup's registers hold."""
+    lens = [20000, 16385, 300, 32768, 31999] + [1500 + 900 * i for i in range(30)]
+    check_select(ctx, heavy(3, len(lens), 2, 32768), lens, 1111, 4, 100)
 
 
 @pytest.mark.parametrize("n", [300, 3000, 40000, 100000])
