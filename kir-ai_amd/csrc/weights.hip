@@ -7,8 +7,12 @@
 // launch merges the splits' outputs and, in other workgroups, turns the scores into weights and
 // adds them to the accumulator:
 //   out[p] = decay in[p] + sum_rows 2^(s - m) / l.
-// Keeping a score costs 8 bytes a (row, key), written and read; computing it again would read K
+// The sums' order is fixed.  Keeping a score costs 8 bytes a (row, key), written and read; computing it again would read K
 // again, 2 head_dim bytes a key: dearer up to 16 rows of a kv head at head_dim 128 in 16 bits.
+//
+// Bound: memory, at the rate of a copy, in large steps; the launch and its loads in small ones.
+// Measured on MI355X (the second launch, us): 32 x U[256, 4096], Hq16 / Hkv8 6.1; 64 x 8192, Hq32 / Hkv8 20.8 (101
+// MB, 4.8 TB/s); one sequence of 512 3.0.
 #include "rows_split.h"
 #include "wave_ops.h"
 
@@ -312,7 +316,11 @@ static hipError_t launch_finish(const RowsArgs &a, int max_len, hipStream_t s) {
 template <int D>
 static hipError_t launch_finish_d(const RowsArgs &a, int max_len, hipStream_t s) {
   const int rows = a.max_rows * (a.q_heads / a.pool.kv_heads);
-  if (rows <= 4) return launch_finish<D, 256, 1, 4, 4>(a, max_len, s);
+  // few rows, a wavefront's positions each its own / shared by four (both launches, us): Hq32 / Hkv8, 1 x 1000 12.5 /
+  // 11.5, 8 x 1000 14.2 / 13.8, 8 x 4000 32.3 / 33.1, 32 x 4000 106.5 / 113.3; eight rows (Hq32 / Hkv4) 1 x 1000
+  // 14.7 / 12.4, 8 x 4000 24.5 / 23.3, 32 x 4000 65.5 / 67.3
+  const long long wgs = (long long)a.num_seqs * a.pool.kv_heads * (((long long)max_len + 1023) / 1024);
+  if (rows <= 4 && wgs >= 128) return launch_finish<D, 256, 1, 4, 4>(a, max_len, s);
   if (rows <= 16) return launch_finish<D, 256, 4, 4, 4>(a, max_len, s);
   return launch_finish<D, 1024, 16, 2, 16>(a, max_len, s);
 }
