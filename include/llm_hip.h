@@ -461,7 +461,8 @@ size_t llh_qk_rope_workspace_bytes(int32_t num_tokens, int32_t num_kv_heads, int
  *                            + sum over the kv head's query heads of weight p    for p < len_b
  * (tokens outside the window receive 0; entries from len_b on are left as they were).
  * d_weights_in, d_weights_out: f32 [num_seqs][kv_heads][weights_stride], weights_stride >=
- * max_seq_len.  d_weights_in = NULL stands for zeros; it may be d_weights_out, no other overlap.
+ * max_seq_len, which is at most 2^28.  d_weights_in = NULL stands for zeros; it may be
+ * d_weights_out, no other overlap.
  * decay must be finite.  The output is llh_paged_decode's within the rounding of the weights;
  * every pool format, head_dim <= 512.  A key in a block outside the pool is masked (and flagged),
  * a query that is left with no key gives a zero row and adds nothing, and a non-finite score
@@ -525,7 +526,8 @@ size_t llh_kv_select_workspace_bytes(int32_t num_seqs, int32_t kv_heads, int32_t
  * and its sequence is left alone. */
 typedef struct llh_kv_compact_desc {
   int32_t num_seqs;
-  int32_t max_kept;        /* host-known bound on d_kept_lens, <= keep_stride, dst_max_blocks * block_tokens */
+  int32_t max_kept;        /* host-known bound on d_kept_lens, <= keep_stride, dst_max_blocks * block_tokens,
+                            * 2^30 tokens and 2^22 blocks */
   int32_t src_max_blocks;  /* row stride of d_src_tables */
   int32_t dst_max_blocks;  /* row stride of d_dst_tables */
   int64_t keep_stride;

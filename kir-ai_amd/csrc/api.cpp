@@ -1360,7 +1360,7 @@ int weights_impl(llh_ctx *ctx, const llh_kv_pool *pool, const WeightsCall &c, co
     return ctx->fail(LLH_ERR_NULL, "null device pointer in attention weights call");
   if (c.num_seqs > 65535 || pool->view.kv_heads > 65535)
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "num_seqs and kv_heads must be <= 65535");
-  if (c.max_ctx > kWeightsMaxLen) return ctx->fail(LLH_ERR_INVALID_SHAPE, "context too long for one call");
+  if (c.max_ctx > kWeightsMaxLen) return ctx->fail(LLH_ERR_INVALID_SHAPE, "attention weights take contexts up to 2^28");
   if (stride < std::max(1, c.max_ctx))
     return ctx->fail(LLH_ERR_INVALID_SHAPE, "weights_stride must hold the longest context");
   if ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 1)

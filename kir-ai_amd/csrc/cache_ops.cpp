@@ -202,6 +202,10 @@ int llh_kv_compact(llh_ctx *ctx, llh_kv_pool *pool, const llh_kv_compact_desc *d
     if (desc->max_kept < 0 || desc->max_kept > desc->keep_stride ||
         desc->max_kept > (int64_t)desc->dst_max_blocks * pv.block_tokens)
       return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_kept must fit keep_stride and the destination rows");
+    // (a launch dimension's threads, 512 a block, and the kernels' 32-bit offsets inside a block)
+    if (((int64_t)desc->max_kept + pv.block_tokens - 1) / pv.block_tokens > kCompactMaxBlocks ||
+        desc->max_kept > kSelectMaxLen || (int64_t)pv.block_tokens * pv.head_dim > (1 << 30))
+      return ctx->fail(LLH_ERR_INVALID_SHAPE, "max_kept must be at most 2^30 tokens in 2^22 blocks");
     if ((desc->d_weights_in == nullptr) != (desc->d_weights_out == nullptr))
       return ctx->fail(LLH_ERR_NULL, "weights are moved from an input to an output: both or neither");
     if (desc->d_weights_in && (desc->weights_in_stride < 0 || desc->weights_out_stride < desc->max_kept))

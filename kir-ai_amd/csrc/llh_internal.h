@@ -220,6 +220,7 @@ struct SelectArgs {
   void *scratch;            // select_scratch_bytes
 };
 constexpr int kSelectMaxLen = 1 << 30;
+constexpr int kCompactMaxBlocks = 1 << 22;
 // bytes of SelectArgs::scratch: 0 where one workgroup holds a row
 size_t select_scratch_bytes(int num_seqs, int kv_heads, int max_seq_len);
 
@@ -341,7 +342,7 @@ hipError_t launch_fp8_encode_check(unsigned long long *mismatches, hipStream_t s
 hipError_t launch_matvec_bf16(const MatvecArgs &a, hipStream_t s);
 // scores, ws_ml (one split) and output of every shape the packed-row kernel does not take (head_dim <= 512)
 constexpr int kWeightsMaxDim = 512;
-constexpr int kWeightsMaxLen = 1 << 30;
+constexpr int kWeightsMaxLen = 1 << 28;  // tiles of 128 positions by 1024 threads stay below 2^32
 hipError_t launch_weights_generic(const RowsArgs &a, hipStream_t s);
 // merges the splits and accumulates
 hipError_t launch_weights_finish(const RowsArgs &a, int max_len, hipStream_t s);

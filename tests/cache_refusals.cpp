@@ -142,6 +142,12 @@ static void weights_cases() {
     c.stride = int64_t{1} << 31;
     c.blocks = 1 << 27;
   });
+  // (tiles of 128 positions by 1024 threads: a launch dimension holds 2^32 threads)
+  weights_case("length past a launch", LLH_ERR_INVALID_SHAPE, [](Weights &c) {
+    c.max_len = (1 << 28) + 1;
+    c.stride = int64_t{1} << 31;
+    c.blocks = 1 << 27;
+  });
   weights_case("weights stride", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.stride = 99; });
   weights_case("empty weights", LLH_ERR_INVALID_SHAPE, [](Weights &c) { c.stride = c.max_len = 0; });
   weights_case("null queries", LLH_ERR_NULL, [](Weights &c) { c.q = nullptr; });
@@ -246,6 +252,17 @@ static void compact_cases() {
   compact_case("negative kept", LLH_ERR_INVALID_SHAPE, [](D &d) { d.max_kept = -1; });
   compact_case("keep stride", LLH_ERR_INVALID_SHAPE, [](D &d) { d.keep_stride = 31; });
   compact_case("destination row", LLH_ERR_INVALID_SHAPE, [](D &d) { d.max_kept = d.keep_stride = 33; });
+  // (the blocks of the largest int, rounded up, pass it; 2^22 blocks of 512 threads are a launch's most)
+  compact_case("kept tokens past an int's blocks", LLH_ERR_INVALID_SHAPE, [](D &d) {
+    d.max_kept = INT32_MAX;
+    d.keep_stride = d.weights_out_stride = int64_t{1} << 31;
+    d.dst_max_blocks = INT32_MAX;
+  });
+  compact_case("kept tokens past a launch", LLH_ERR_INVALID_SHAPE, [](D &d) {
+    d.max_kept = (1 << 26) + 1;
+    d.keep_stride = d.weights_out_stride = int64_t{1} << 31;
+    d.dst_max_blocks = INT32_MAX;
+  });
   compact_case("weights in alone", LLH_ERR_NULL, [](D &d) { d.d_weights_out = nullptr; });
   compact_case("weights out alone", LLH_ERR_NULL, [](D &d) { d.d_weights_in = nullptr; });
   compact_case("weights out stride", LLH_ERR_INVALID_SHAPE, [](D &d) { d.weights_out_stride = 31; });
