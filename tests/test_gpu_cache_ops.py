@@ -140,6 +140,42 @@ def test_norm_rope_in_place(ctx):
         assert torch.equal(k.view(torch.int16), ko.view(torch.int16))
 
 
+@pytest.mark.parametrize("n,Hq,Hkv,D,R,adjacent", [
+    # prompts, whose workgroups take several heads of their tokens: odd counts, both pairings
+    (1037, 16, 8, 128, 128, False), (1024, 5, 1, 128, 128, True), (1041, 32, 4, 128, 64, False),
+    (1029, 3, 1, 128, 2, True), (1037, 16, 2, 256, 64, False), (1025, 9, 2, 256, 256, True), (1031, 4, 2, 64, 64, False),
+    # more heads than a workgroup's wavefronts load at once
+    (5, 64, 8, 128, 128, False), (2, 96, 96, 128, 64, True), (3, 40, 8, 256, 64, False), (2, 64, 2, 256, 256, True),
+])
+@pytest.mark.parametrize("off", [0, 1])
+def test_norm_rope_many_rows(ctx, n, Hq, Hkv, D, R, adjacent, off):
+    """Against the formula, written elsewhere and over the input; off: outputs off their 16 bytes."""
+    import torch
+
+    qkv, wq, wk, pos, freq = rope_case(n, Hq, Hkv, D, R, 31 + D + n)
+    t = view_bf16(qkv)
+    q, k, _ = split(t, Hq, Hkv, D)
+    dev = [view_bf16(wq), view_bf16(wk), to_dev(pos), to_dev(freq)]
+    d = ctx.qk_rope_desc(q, k, None, dev[2], dev[3], q_weight=dev[0], k_weight=dev[1], adjacent=adjacent)
+    outs = [torch.full((n * H * D + 2,), math.nan, dtype=torch.bfloat16, device="cuda") for H in (Hq, Hkv)]
+    qo, ko = (o[off:off + n * H * D].view(n, H, D) for o, H in zip(outs, (Hq, Hkv)))
+    ctx.qk_norm_rope(d, qo, ko)
+    torch.cuda.synchronize()
+    assert ctx.device_errors() == 0
+    for name, out, x, w in (("q", qo, q, wq), ("k", ko, k, wk)):
+        want = ref.norm_rope(x.float().cpu().numpy(), pos, freq, f(w), 0.0, 1e-6, adjacent)
+        top = np.abs(want).max(-1, keepdims=True)
+        assert_rounded(from_dev_bf16(out.contiguous().view(torch.int16)), want, top, name)
+    for o, H in zip(outs, (Hq, Hkv)):  # nothing beside the rows
+        assert o[:off].isnan().all() and o[off + n * H * D:].isnan().all()
+    if off == 0:
+        qc, kc = q.contiguous(), k.contiguous()
+        ctx.qk_norm_rope(ctx.qk_rope_desc(qc, kc, None, dev[2], dev[3], q_weight=dev[0], k_weight=dev[1],
+                                          adjacent=adjacent), qc, kc)
+        assert torch.equal(qc.view(torch.int16), qo.view(torch.int16))
+        assert torch.equal(kc.view(torch.int16), ko.view(torch.int16))
+
+
 def fresh_pool(ctx, fmt, bt, hkv, d, n, seed):
     """A pool whose blocks all hold rows."""
     pool = ctx.pool(fmt, bt, hkv, d, n)
@@ -167,6 +203,41 @@ def test_norm_rope_append_is_the_two_calls(ctx, fmt, Hq, Hkv, D, bt, pad):
     dev = [view_bf16(wq), view_bf16(wk), to_dev(pos), to_dev(freq), to_dev(slots)]
     d = ctx.qk_rope_desc(q, k, v, dev[2], dev[3], q_weight=dev[0], k_weight=dev[1])
     one, two = (fresh_pool(ctx, ALL_FMTS[fmt], bt, Hkv, D, 14, 90) for _ in range(2))
+    q1, q2 = (torch.full((n, Hq, D), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k2 = torch.empty((n, Hkv, D), dtype=torch.bfloat16, device="cuda")
+    ctx.qk_norm_rope_append(one, d, dev[4], q1)
+    ctx.qk_norm_rope(d, q2, k2)
+    ctx.append(two, dev[4], k2, v.contiguous())
+    torch.cuda.synchronize()
+    assert ctx.device_errors() == 0
+    assert torch.equal(q1.view(torch.int16), q2.view(torch.int16))
+    a, b = one.raw(), two.raw()
+    for key in a:
+        assert np.array_equal(a[key], b[key]), key
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16", "int8", "fp8"])
+@pytest.mark.parametrize("n,Hq,Hkv,D", [(1037, 16, 8, 128), (1030, 16, 2, 256), (1026, 5, 1, 128), (35, 64, 8, 128),
+                                        (33, 40, 8, 256)])
+def test_norm_rope_append_many_rows(ctx, fmt, n, Hq, Hkv, D):
+    """Prompts of several sequences, which start and end inside blocks, and many heads."""
+    import torch
+
+    rng = np.random.default_rng(n)
+    blocks = rng.permutation(-(-n // BT) + 8)
+    slots, at = [], 0
+    for length in (n // 3, 1, n - n // 3 - 1):  # each from some offset of its own blocks
+        first = int(rng.integers(0, BT))
+        rows = np.arange(first, first + length)
+        slots.append(blocks[at + rows // BT] * BT + rows % BT)
+        at += rows[-1] // BT + 1
+    slots = np.concatenate(slots).astype(np.int64)
+    assert slots.size == n and np.unique(slots).size == n and at <= blocks.size
+    qkv, wq, wk, pos, freq = rope_case(n, Hq, Hkv, D, D, 4)
+    q, k, v = split(view_bf16(qkv), Hq, Hkv, D)
+    dev = [view_bf16(wq), view_bf16(wk), to_dev(pos), to_dev(freq), to_dev(slots)]
+    d = ctx.qk_rope_desc(q, k, v, dev[2], dev[3], q_weight=dev[0], k_weight=dev[1])
+    one, two = (fresh_pool(ctx, FMTS[fmt], BT, Hkv, D, blocks.size, 92) for _ in range(2))
     q1, q2 = (torch.full((n, Hq, D), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(2))
     k2 = torch.empty((n, Hkv, D), dtype=torch.bfloat16, device="cuda")
     ctx.qk_norm_rope_append(one, d, dev[4], q1)
@@ -364,6 +435,16 @@ def test_decode_weights_splits(ctx, fmt, Hq, Hkv, D):
     """One long sequence in many splits beside short ones, gated."""
     check_weights(ctx, fmt, [9000, 3, 1500], Hq, Hkv, D, gate=True)
     check_weights(ctx, fmt, [4097], Hq, Hkv, D, window=2049)
+
+
+@pytest.mark.parametrize("window", [0, 129])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 128), (32, 8, 128), (8, 8, 256), (24, 8, 128)])
+def test_decode_weights_of_many_sequences(ctx, Hq, Hkv, D, fmt, window):
+    """Few rows of many kv heads, whose weights a wavefront adds up alone, over ends at every side of
+    its 256 positions."""
+    lens = [255, 256, 257, 0, 1, 321, 511, 512, 513, 767, 769, 1023, 1024, 1025, 1100, 3, 64, 700, 900, 400]
+    check_weights(ctx, fmt, lens, Hq, Hkv, D, window, gate=True)
 
 
 @pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 128), (16, 2, 256), (4, 2, 64)])
