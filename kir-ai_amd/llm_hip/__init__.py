@@ -799,7 +799,7 @@ class Context:
                              weights_out, decay: float = 1.0, stream=None) -> None:
         """llh_paged_decode_weights: a decode step that adds each token's softmax weight to the accumulator,
         f32 [num_seqs][kv_heads][stride]; weights_in: None (zeros), another tensor or weights_out itself."""
-        self._check_weights(weights_in, weights_out)
+        self._check_weights(pool, desc, weights_in, weights_out)
         self.check(self.lib.llh_paged_decode_weights(
             self.handle, pool.handle, ctypes.byref(desc), _ptr(q), _ptr(out), score_scale, _ptr(weights_in),
             _ptr(weights_out), weights_out.shape[-1], decay, self._own_stream(stream)))
@@ -807,18 +807,27 @@ class Context:
     def paged_prefill_weights(self, pool: "KvPool", desc: PrefillDesc, max_context_len: int, q, out,
                               score_scale: float, weights_in, weights_out, decay: float = 1.0, stream=None) -> None:
         """llh_paged_prefill_weights: the same for each sequence's last rows (at most WEIGHTS_MAX_CHUNK)."""
-        self._check_weights(weights_in, weights_out)
+        self._check_weights(pool, desc, weights_in, weights_out)
         self.check(self.lib.llh_paged_prefill_weights(
             self.handle, pool.handle, ctypes.byref(desc), max_context_len, _ptr(q), _ptr(out), score_scale,
             _ptr(weights_in), _ptr(weights_out), weights_out.shape[-1], decay, self._own_stream(stream)))
 
     @staticmethod
-    def _check_weights(weights_in, weights_out) -> None:
+    def _check_weights(pool, desc, weights_in, weights_out) -> None:
         import torch
 
         for w in (weights_in, weights_out):
             if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or w.shape != weights_out.shape):
                 raise LlhError(ERR_INVALID_SHAPE, "weights are contiguous f32 of one shape")
+        if weights_out.dim() != 3 or tuple(weights_out.shape[:2]) != (desc.num_seqs, pool.info.kv_heads):
+            raise LlhError(ERR_INVALID_SHAPE, "weights are [num_seqs][kv_heads][stride]")
+
+    @staticmethod
+    def _check_rows(what: str, dtype, *tensors) -> None:
+        """Rows that the library walks by their element count."""
+        for x in tensors:
+            if x is not None and (x.dtype != dtype or not x.is_contiguous()):
+                raise LlhError(ERR_INVALID_SHAPE, f"{what} are contiguous {dtype}")
 
     def select_workspace_bytes(self, num_seqs: int, kv_heads: int, max_seq_len: int) -> int:
         return self.lib.llh_kv_select_workspace_bytes(num_seqs, kv_heads, max_seq_len)
@@ -842,6 +851,14 @@ class Context:
 
     def kv_select(self, desc: KvSelectDesc, weights, keep, kept_lens, stream=None) -> None:
         """llh_kv_select: the positions each (sequence, kv head) keeps, ascending, and the lengths that leaves."""
+        import torch
+
+        self._check_rows("weights", torch.float32, weights)
+        self._check_rows("positions and lengths", torch.int32, keep, kept_lens)
+        rows = desc.num_seqs * desc.kv_heads
+        if weights.numel() < rows * desc.weights_stride or keep.numel() < rows * desc.keep_stride or (
+                kept_lens.numel() < desc.num_seqs):
+            raise LlhError(ERR_INVALID_SHAPE, "weights, positions and lengths of every (sequence, kv head)")
         self.check(self.lib.llh_kv_select(self.handle, ctypes.byref(desc), _ptr(weights), _ptr(keep),
                                           _ptr(kept_lens), self._own_stream(stream)))
 
@@ -850,6 +867,17 @@ class Context:
                      weights_out=None) -> KvCompactDesc:
         """Descriptor of llh_kv_compact over device tensors (kept alive): keep int32 [num_seqs][kv_heads][stride],
         tables int32 [num_seqs][blocks], weights f32 [num_seqs][kv_heads][stride] or None."""
+        import torch
+
+        Context._check_rows("positions, lengths and tables", torch.int32, seq_lens, kept_lens, keep, src_tables,
+                            dst_tables)
+        Context._check_rows("weights", torch.float32, weights_in, weights_out)
+        n = seq_lens.shape[0]
+        if kept_lens.numel() != n or any(x is not None and (x.dim() != d or x.shape[0] != n) for x, d in (
+                (keep, 3), (src_tables, 2), (dst_tables, 2), (weights_in, 3), (weights_out, 3))):
+            raise LlhError(ERR_INVALID_SHAPE, "one row of positions, lengths and tables a sequence")
+        if any(w is not None and w.shape[1] != keep.shape[1] for w in (weights_in, weights_out)):
+            raise LlhError(ERR_INVALID_SHAPE, "weights of the kept heads")
         d = KvCompactDesc(
             num_seqs=seq_lens.shape[0],
             max_kept=max_kept,
@@ -871,6 +899,8 @@ class Context:
 
     def kv_compact(self, pool: "KvPool", desc: KvCompactDesc, stream=None) -> None:
         """llh_kv_compact: the kept tokens (and their weights) to the destination tables' blocks."""
+        if getattr(desc, "_keep", None) and desc._keep[2].shape[1] != pool.info.kv_heads:
+            raise LlhError(ERR_INVALID_SHAPE, "positions are [num_seqs][kv_heads][stride]")
         self.check(self.lib.llh_kv_compact(self.handle, pool.handle, ctypes.byref(desc), self._own_stream(stream)))
 
     def write_blocks(self, pool: "KvPool", blocks, k, v, stream=None) -> None:

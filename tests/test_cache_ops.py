@@ -62,3 +62,45 @@ def test_workspace_bound():
     assert lib.llh_weights_workspace_bytes(4, 1, 16, 128, 1000) >= 4 * 16 * 1000 * 4
     assert lib.llh_weights_workspace_bytes(4, 8, 16, 128, 1000) >= 8 * 4 * 16 * 1000 * 4
     assert lib.llh_weights_workspace_bytes(4, 0, 16, 128, 1000) == 0
+
+
+def test_binding_refuses_rows_it_would_misread():
+    """Tensors of another shape, type or order than the library walks, before any call reaches it."""
+    import types
+
+    import pytest
+    import torch
+
+    ctx = llm_hip.Context.__new__(llm_hip.Context)
+    ctx.handle = None  # nothing below gets as far as the library
+    i32 = dict(dtype=torch.int32)
+    pool = types.SimpleNamespace(info=types.SimpleNamespace(kv_heads=4), handle=None)
+    lens, w = torch.zeros(2, **i32), torch.zeros(2, 4, 64)
+    desc = types.SimpleNamespace(num_seqs=2)
+    ctx._check_weights(pool, desc, None, w)
+    ctx._check_weights(pool, desc, w, w)
+    for w_in, w_out in [(None, w[:1]), (None, w[:, :2].contiguous()), (None, w.reshape(8, 64)), (w[..., :32], w),
+                        (None, w.double()), (None, w.transpose(0, 1)), (w[:1], w)]:
+        with pytest.raises(llm_hip.LlhError):
+            ctx._check_weights(pool, desc, w_in, w_out)
+
+    keep, kept = torch.zeros(2, 4, 16, **i32), torch.zeros(2, **i32)
+    select = ctx.select_desc(lens, 4, 64, 16, 0, 0, 64, 16)
+    for bad in [dict(weights=w[:1]), dict(weights=w.half()), dict(weights=w[..., ::2]), dict(keep=keep[:, :3].contiguous()),
+                dict(keep=keep.long()), dict(keep=keep.transpose(0, 1)), dict(kept_lens=kept[:1]),
+                dict(kept_lens=kept.long())]:
+        with pytest.raises(llm_hip.LlhError):
+            ctx.kv_select(select, **dict(dict(weights=w, keep=keep, kept_lens=kept), **bad))
+
+    good = dict(seq_lens=lens, kept_lens=kept, keep=keep, src_tables=torch.zeros(2, 4, **i32),
+                dst_tables=torch.zeros(2, 1, **i32), max_kept=16, weights_in=w, weights_out=w.clone())
+    move = ctx.compact_desc(**good)
+    for bad in [dict(keep=keep[0]), dict(keep=keep[:1]), dict(keep=keep.long()), dict(kept_lens=kept[:1]),
+                dict(src_tables=good["src_tables"].long()), dict(src_tables=good["src_tables"][:, ::2]),
+                dict(dst_tables=good["dst_tables"][:1]), dict(weights_in=w.double()),
+                dict(weights_out=torch.zeros(2, 2, 64)), dict(weights_in=w[0])]:
+        with pytest.raises(llm_hip.LlhError):
+            ctx.compact_desc(**dict(good, **bad))
+    pool.info.kv_heads = 2
+    with pytest.raises(llm_hip.LlhError):
+        ctx.kv_compact(pool, move)
